@@ -1,0 +1,57 @@
+// Shared declarations of the context attention kernels: attention of query tokens to states of another length
+// (an encoder's text / audio / image states, a cached clip), with per-sample lengths, packed samples, key masks and
+// grouped heads. context_attn_tc.cu has the tensor-memory kernel for full query tiles, context_attn_rows.cu the kernel
+// for a few query rows and the join of partial results, context_attn_host.cu picks between them.
+#pragma once
+#include "tfb_api.h"
+#include "tfb_common.cuh"
+#include "tfb_host.h"
+
+namespace tfb {
+
+struct CtxParams {
+  const void *q, *k, *v;
+  long q_bs, q_ss, q_hs, k_bs, k_ss, k_hs, v_bs, v_ss, v_hs;  // element strides of batch, token, head
+  void* out;        // [B, Sq, H, D] contiguous
+  float* lse;       // [B, H, Sq] or null
+  float* part_o;    // non-null: results go to slots [slot][B * Sq][H][D] (each slot normalised by its own sum) ...
+  float* part_lse;  // ... with base-2 log-sum-exps [slot][B * Sq][H]; -inf marks a slot that saw no key (its part_o is not written)
+  const int* kv_lens;
+  const int* cu_kv;
+  const uint8_t* key_mask;
+  long mask_bs;
+  int B, Sq, H, Hkv, D, Skv, P;  // Skv: rows of k / v per sample (all rows when packed); P: rows of the prefix
+  int ns, slot0;                 // key range split over ns slots, the first of them slot0
+  float scale_log2;
+  int* status;
+};
+
+// Rows [first, first + len) of the sample's own keys. Lengths and offsets come from device memory, so they are clamped
+// here: no value of theirs can lead outside the tensors.
+__device__ __forceinline__ void ctx_sample_range(const CtxParams& p, int b, int& first, int& len) {
+  if (p.cu_kv) {
+    const int a = __ldg(p.cu_kv + b), e = __ldg(p.cu_kv + b + 1);
+    first = min(max(a, 0), p.Skv);
+    len = max(min(e, p.Skv) - first, 0);
+  } else {
+    first = 0;
+    len = p.kv_lens ? min(max(__ldg(p.kv_lens + b), 0), p.Skv) : p.Skv;
+  }
+}
+
+template <bool FP16>
+__device__ __forceinline__ uint32_t ctx_pack2(float lo, float hi) {
+  return FP16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
+}
+
+// Few query rows (Sq * H / Hkv <= 16) of every sample against its own keys.
+int launch_ctx_rows(const CtxParams& p, int fp16, cudaStream_t st);
+// Joins p.ns slots of part_o / part_lse (slot0 = 0) into out and lse.
+int launch_ctx_join(const CtxParams& p, int fp16, cudaStream_t st);
+// Full query tiles. kp / vp: the shared prefix (p.P rows, strides in elements), visited before the sample's own keys.
+int launch_ctx_tc(const CtxParams& p, const void* kp, long kp_ss, long kp_hs, const void* vp, long vp_ss, long vp_hs,
+                  int fp16, cudaStream_t st);
+// Work items of launch_ctx_tc with p.ns = 1.
+long ctx_tc_items(int B, int Sq, int H, int Hkv);
+
+}  // namespace tfb

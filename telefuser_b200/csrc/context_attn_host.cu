@@ -1,0 +1,134 @@
+// C entry points of context attention: argument checks, the choice of kernels and key splits.
+//
+// Rows kernel (context_attn_rows.cu) when a sample has at most 16 query rows per key head, tensor-memory kernel
+// (context_attn_tc.cu) otherwise. A shared prefix is visited by the tensor-memory kernel as the first key blocks of every
+// sample when the sample fills a query tile; below that the prefix is computed once for all samples - their tokens form
+// one batch entry - as slots of its own, the samples' own keys as further slots, and the join adds them up.
+#include "context_attn.cuh"
+
+using namespace tfb;
+
+namespace {
+
+constexpr int CTX_MAX_SPLITS = 64;
+
+struct CtxPlan {
+  bool apart;          // prefix in slots of its own
+  int ns_prefix, ns;   // key splits of the prefix pass and of the (only or own-keys) pass
+  bool rows_prefix, rows_own;
+  int slots() const { return (apart ? ns_prefix : 0) + ns; }
+};
+
+bool few_rows(long tokens, int H, int Hkv) { return tokens * (H / Hkv) <= 16; }
+
+// Splits of the key range so that few items still fill the device: about three CTAs per SM for the rows kernel (three
+// are resident), one per SM for the tensor-memory kernel; a slice is never shorter than what a CTA takes in one step.
+int pick_splits(bool rows, int B, long Sq, int H, int Hkv, long keys) {
+  const long sms = sm_count();
+  const long items = rows ? static_cast<long>(B) * Hkv : ctx_tc_items(B, static_cast<int>(Sq), H, Hkv);
+  long ns = (rows ? 3 * sms : sms) / (items > 0 ? items : 1);
+  const long most = (keys + 127) / 128 / (rows ? 1 : 2);
+  if (ns > most) ns = most;
+  if (ns > CTX_MAX_SPLITS) ns = CTX_MAX_SPLITS;
+  return ns < 1 ? 1 : static_cast<int>(ns);
+}
+
+int check(const tfb_context_attn_args* a) {
+  if (!a || a->B < 0 || a->Sq < 0 || a->H < 1 || a->Hkv < 1 || a->H % a->Hkv || a->D < 8 || a->D > 128 || a->D % 8 ||
+      a->Skv < 0 || a->P < 0 || !(a->scale > 0.f))
+    return TFB_ERR_BAD_SHAPE;
+  if ((a->cu_kv && (a->kv_lens || a->key_mask)) || (a->P && (a->cu_kv || a->key_mask))) return TFB_ERR_BAD_SHAPE;
+  if (a->Sq > (1 << 30) || a->Skv > (1 << 30) || a->P > (1 << 30)) return TFB_ERR_TOO_LARGE;
+  return TFB_OK;
+}
+
+CtxPlan make_plan(const tfb_context_attn_args* a) {
+  CtxPlan pl;
+  const int G = a->H / a->Hkv;
+  pl.apart = a->P > 0 && static_cast<long>(a->Sq) * G < 128;
+  pl.rows_own = few_rows(a->Sq, a->H, a->Hkv) && (a->P == 0 || pl.apart);
+  const long tokens = static_cast<long>(a->B) * a->Sq;
+  pl.rows_prefix = few_rows(tokens, a->H, a->Hkv);
+  // Packed samples: the longest may hold every row.
+  const long keys = a->Skv + (pl.apart ? 0 : a->P);
+  pl.ns = pick_splits(pl.rows_own, a->B, a->Sq, a->H, a->Hkv, keys);
+  pl.ns_prefix = pl.apart ? pick_splits(pl.rows_prefix, 1, tokens, a->H, a->Hkv, a->P) : 0;
+  return pl;
+}
+
+}  // namespace
+
+extern "C" long tfb_context_attn_work(const tfb_context_attn_args* a) {
+  if (int e = check(a)) return -e;
+  if (a->B == 0 || a->Sq == 0) return 0;
+  const CtxPlan pl = make_plan(a);
+  if (pl.slots() == 1) return 0;
+  return static_cast<long>(pl.slots()) * a->B * a->Sq * a->H * (a->D + 1) * static_cast<long>(sizeof(float));
+}
+
+extern "C" int tfb_context_attn(const tfb_context_attn_args* a, void* stream) {
+  if (int e = check(a)) return e;
+  if (a->B == 0 || a->Sq == 0) return TFB_OK;
+  if ((a->q_bs | a->q_ss | a->q_hs | a->k_bs | a->k_ss | a->k_hs | a->v_bs | a->v_ss | a->v_hs | a->kp_ss | a->kp_hs |
+       a->vp_ss | a->vp_hs) % 8)
+    return TFB_ERR_BAD_SHAPE;
+  if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v) |
+       reinterpret_cast<uintptr_t>(a->kp) | reinterpret_cast<uintptr_t>(a->vp) | reinterpret_cast<uintptr_t>(a->out) |
+       reinterpret_cast<uintptr_t>(a->work)) & 15)
+    return TFB_ERR_BAD_SHAPE;
+  if (!a->q || !a->out || (a->Skv && (!a->k || !a->v)) || (a->P && (!a->kp || !a->vp))) return TFB_ERR_BAD_SHAPE;
+  const CtxPlan pl = make_plan(a);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  CtxParams p;
+  p.q = a->q, p.k = a->k, p.v = a->v;
+  p.q_bs = a->q_bs, p.q_ss = a->q_ss, p.q_hs = a->q_hs;
+  p.k_bs = a->k_bs, p.k_ss = a->k_ss, p.k_hs = a->k_hs;
+  p.v_bs = a->v_bs, p.v_ss = a->v_ss, p.v_hs = a->v_hs;
+  p.out = a->out;
+  p.lse = a->lse;
+  p.kv_lens = a->kv_lens;
+  p.cu_kv = a->cu_kv;
+  p.key_mask = static_cast<const uint8_t*>(a->key_mask);
+  p.mask_bs = a->mask_bs;
+  p.B = a->B, p.Sq = a->Sq, p.H = a->H, p.Hkv = a->Hkv, p.D = a->D, p.Skv = a->Skv;
+  p.P = pl.apart ? 0 : a->P;
+  p.ns = pl.ns;
+  p.slot0 = pl.apart ? pl.ns_prefix : 0;
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.status = status_word();
+  p.part_o = p.part_lse = nullptr;
+  if (pl.slots() > 1) {
+    if (!a->work) return TFB_ERR_BAD_SHAPE;
+    p.part_o = a->work;
+    p.part_lse = a->work + static_cast<long>(pl.slots()) * a->B * a->Sq * a->H * a->D;
+  }
+  if (pl.apart) {
+    // All samples' tokens as one batch entry: needs one stride from token to token.
+    const long ss = a->Sq == 1 ? a->q_bs : a->q_ss;
+    if (a->B > 1 && a->Sq > 1 && a->q_bs != a->Sq * a->q_ss) return TFB_ERR_BAD_SHAPE;
+    const long tokens = static_cast<long>(a->B) * a->Sq;
+    if (tokens > (1 << 30)) return TFB_ERR_TOO_LARGE;
+    CtxParams f = p;
+    f.q_ss = a->B > 1 ? ss : a->q_ss;
+    f.q_bs = 0;
+    f.k = a->kp, f.v = a->vp;
+    f.k_bs = f.v_bs = 0;
+    f.k_ss = a->kp_ss, f.k_hs = a->kp_hs, f.v_ss = a->vp_ss, f.v_hs = a->vp_hs;
+    f.kv_lens = nullptr;
+    f.B = 1, f.Sq = static_cast<int>(tokens), f.Skv = a->P;
+    f.ns = pl.ns_prefix;
+    f.slot0 = 0;
+    if (int e = pl.rows_prefix ? launch_ctx_rows(f, a->fp16, st)
+                               : launch_ctx_tc(f, nullptr, 0, 0, nullptr, 0, 0, a->fp16, st))
+      return e;
+  }
+  if (int e = pl.rows_own
+                  ? launch_ctx_rows(p, a->fp16, st)
+                  : launch_ctx_tc(p, a->kp, a->kp_ss, a->kp_hs, a->vp, a->vp_ss, a->vp_hs, a->fp16, st))
+    return e;
+  if (pl.slots() > 1) {
+    p.ns = pl.slots();
+    return launch_ctx_join(p, a->fp16, st);
+  }
+  return TFB_OK;
+}

@@ -262,6 +262,39 @@ int tfb_plucker_fold(const float* c2w, const float* ks, const float* extra, int 
 // frames [3, T, H, W] (fp32 or bf16) in [-1, 1] -> uint8 [T, H, W, 3].  W % 4 == 0.
 int tfb_frames_to_u8(const void* frames, int is_bf16, void* out, int T, int H, int W, void* stream);
 
+// ---- context attention (context_attn_host.cu, context_attn_tc.cu, context_attn_rows.cu) ----
+// softmax(scale q k^T) v of Sq query tokens against P shared prefix rows followed by the sample's own rows, head_dim D a
+// multiple of 8 up to 128, H a multiple of Hkv, bf16 or fp16, all strides in elements and multiples of 8, 16-byte bases.
+// Own rows of sample b: [0, kv_lens[b]) of k / v [B, Skv, Hkv, D] (kv_lens null: all Skv), minus those whose
+// key_mask[b * mask_bs + j] is 0; or, with cu_kv, rows [cu_kv[b], cu_kv[b + 1]) of k / v [Skv, Hkv, D]. Lengths and
+// offsets are clamped to the tensors. cu_kv excludes kv_lens and key_mask; a prefix excludes cu_kv and key_mask.
+// out [B, Sq, H, D] contiguous; lse fp32 [B, H, Sq] or null (natural log; -inf and a zero row where no key is visible).
+typedef struct {
+  const void *q, *k, *v, *kp, *vp;
+  void* out;
+  float* lse;
+  const int *kv_lens, *cu_kv;
+  const void* key_mask;
+  float* work;  // tfb_context_attn_work() bytes, 16-byte aligned; null when that is 0
+  long q_bs, q_ss, q_hs, k_bs, k_ss, k_hs, v_bs, v_ss, v_hs, kp_ss, kp_hs, vp_ss, vp_hs, mask_bs;
+  int B, Sq, H, Hkv, D, Skv, P, fp16;
+  float scale;
+  int reserved;
+} tfb_context_attn_args;
+// Bytes of scratch that the call needs (partial results of a split key range), or a negative TFB_ERR_* code.
+long tfb_context_attn_work(const tfb_context_attn_args* a);
+int tfb_context_attn(const tfb_context_attn_args* a, void* stream);
+
+// ---- sandwich norm (sandwich_norm.cu) ----
+// x = res + g * (post ? w * y / rms(y) : y), g = tanh(gate) or gate (1 when null); h = w2 * x / rms(x) * (1 + scale) + shift,
+// computed from x as it is stored. res / y / x / h: bf16 (dtype 0), fp16 (1) or fp32 (2), rows of C elements, C a multiple
+// of 8 up to 8192, 16-byte rows. w / w2: [C] or null, of the activations' type (w_f32 = 0) or fp32 (1). Tables fp32, each
+// with its own row stride and rows per table row (row r reads table row r / rows_per).
+int tfb_sandwich_norm(const void* res, long ldr, const void* y, long ldy, void* x, void* h, long rows, int C, float eps,
+                      int dtype, int w_f32, const void* w, const void* w2, const float* gate, long ldg, long rpg,
+                      const float* shift, long lds, long rps, const float* scale, long ldc, long rpc, int post,
+                      int tanh_gate, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,228 @@
+"""Attention of query tokens to a context of another length: an encoder's states (`cross_attention`) or a cached clip that
+the whole batch shares followed by each sample's own tokens (`prefix_attention`).
+
+Beyond `functional.attention` these take what conditioning brings along: samples of different lengths (padded, packed one
+after the other, or masked), grouped heads without repeating K / V, and one copy of a shared prefix. Layout BSHD as there.
+CUDA bf16 / fp16 tensors with a head dim that is a multiple of 8 up to 128 run on the kernels of `csrc/context_attn_*.cu`;
+everything else (CPU, fp32, other head dims) takes the fp32 evaluation of `context_attention_reference`, in query blocks.
+
+A query that sees no key gives a zero row, and -inf as its log-sum-exp. What lies in padded or masked places does not
+matter, infinities and NaN included. Inference only: no gradient is recorded. Neither call synchronises with the host when
+lengths are given as device tensors, so both can be captured in a CUDA graph.
+
+Role parity: telefuser/ops/attention/attention_impl.py:112-315 (variable-length forms of the attention back ends).
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import native
+from .functional import _native
+
+_NAMES = ("q", "k", "v", "kp", "vp", "out", "lse", "kv_lens", "cu_kv", "key_mask", "work")
+_LONGS = ("q_bs", "q_ss", "q_hs", "k_bs", "k_ss", "k_hs", "v_bs", "v_ss", "v_hs", "kp_ss", "kp_hs", "vp_ss", "vp_hs", "mask_bs")
+_INTS = ("B", "Sq", "H", "Hkv", "D", "Skv", "P", "fp16")
+
+
+class _Args(ctypes.Structure):
+    """tfb_context_attn_args of csrc/tfb_api.h."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in _NAMES] + [(n, ctypes.c_long) for n in _LONGS]
+                + [(n, ctypes.c_int) for n in _INTS] + [("scale", ctypes.c_float), ("reserved", ctypes.c_int)])  # fmt: skip
+
+
+def context_attention_reference(q, k, v, visible=None, scale=None, return_lse=False, q_block: int | None = None):
+    """fp32 evaluation: q [B, Sq, H, D], k / v [B, Skv, Hkv, D] (H a multiple of Hkv), visible bool [B, Skv] or None."""
+    B, Sq, H, D = q.shape
+    Skv, Hkv = k.shape[1], k.shape[2]
+    scale = 1.0 / math.sqrt(D) if scale is None else scale
+    kf, vf = k.float().permute(0, 2, 3, 1), v.float().transpose(1, 2)  # [B, Hkv, D, Skv], [B, Hkv, Skv, D]
+    if visible is not None:  # hidden rows may hold anything
+        kf = kf.masked_fill(~visible[:, None, None, :], 0.0)
+        vf = vf.masked_fill(~visible[:, None, :, None], 0.0)
+    out = torch.empty(B, Sq, H, D, device=q.device, dtype=q.dtype)
+    lse = torch.empty(B, H, Sq, device=q.device, dtype=torch.float32)
+    step = q_block or max(Sq, 1)
+    for s0 in range(0, Sq, step):
+        qf = q[:, s0 : s0 + step].float()
+        n = qf.shape[1]
+        qf = qf.reshape(B, n, Hkv, H // Hkv, D).permute(0, 2, 3, 1, 4).reshape(B, Hkv, -1, D)
+        s = (qf @ kf) * scale
+        if visible is not None:
+            s = s.masked_fill(~visible[:, None, None, :], float("-inf"))
+        ls = torch.logsumexp(s, dim=-1) if Skv else s.new_full(s.shape[:-1], float("-inf"))
+        p = torch.exp(s - ls.masked_fill(ls == float("-inf"), 0.0)[..., None])
+        out[:, s0 : s0 + n] = (p @ vf).reshape(B, H, n, D).transpose(1, 2).to(q.dtype)
+        lse[:, :, s0 : s0 + n] = ls.reshape(B, H, n)
+    return (out, lse) if return_lse else out
+
+
+def _q_block(q, keys: int) -> int | None:
+    return max(128, (1 << 24) // max(keys, 1)) if q.is_cuda and q.shape[1] * keys > (1 << 24) else None
+
+
+def _check(q, k, v, what: str) -> None:
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
+        raise ValueError(f"{what}: q [B, Sq, H, D] and k / v of one shape [B, Skv, Hkv, D], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if k.shape[3] != q.shape[3] or k.shape[2] < 1 or q.shape[2] % k.shape[2]:
+        raise ValueError(f"{what}: heads {q.shape[2]} x {q.shape[3]} do not fit key heads {k.shape[2]} x {k.shape[3]}")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"{what}: q, k and v have one type, got {q.dtype}, {k.dtype}, {v.dtype}")
+    native.same_device(q, k, v)
+
+
+def _scale(scale, D: int) -> float:
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError("the score scale must be positive and finite")
+    return scale
+
+
+def _lengths(lens, n: int, most: int, device, what: str):
+    """-> int32 [n] on `device`. Values that the host holds are checked; values on the device are clamped by the kernels."""
+    if not torch.is_tensor(lens) or lens.device.type == "cpu":
+        values = [int(x) for x in lens]
+        if len(values) != n or any(not 0 <= x <= most for x in values):
+            raise ValueError(f"{what}: {n} values in [0, {most}] expected, got {values}")
+        return torch.tensor(values, dtype=torch.int32, device=device)
+    if lens.shape != (n,) or lens.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what}: an integer tensor of shape ({n},) expected, got {lens.dtype} {tuple(lens.shape)}")
+    if lens.device != device:
+        raise ValueError(f"{what} is on {lens.device}, the queries are on {device}")
+    return lens.contiguous() if lens.dtype == torch.int32 else lens.clamp(-1, 2**31 - 1).to(torch.int32)
+
+
+def _strided(t):
+    """t with unit channel stride, 16-byte rows and no broadcast dimension, copied only if it is not so already."""
+    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0
+    for n, s in zip(t.shape[:-1], t.stride()[:-1]):
+        ok = ok and (n <= 1 or (s > 0 and s % 8 == 0))
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _stride(t, dim: int) -> int:
+    return t.stride(dim) if t.shape[dim] > 1 else 0
+
+
+def _runs_native(q) -> bool:
+    return _native(q) and q.dtype in (torch.bfloat16, torch.float16) and q.shape[3] % 8 == 0 and 8 <= q.shape[3] <= 128
+
+
+def _launch(q, k, v, kp, vp, kv_lens, cu_kv, key_mask, scale, return_lse):
+    if q.device.index != torch.cuda.current_device():
+        with torch.cuda.device(q.device):
+            return _launch(q, k, v, kp, vp, kv_lens, cu_kv, key_mask, scale, return_lse)
+    B, Sq, H, D = q.shape
+    a = _Args()
+    if B > 1 and Sq > 1 and kp is not None and q.stride(0) != Sq * q.stride(1):
+        q = q.contiguous()  # the shared prefix sees the tokens of all samples as one row after the other
+    q, k, v = _strided(q), _strided(k), _strided(v)
+    a.q, a.q_bs, a.q_ss, a.q_hs = q.data_ptr(), _stride(q, 0), _stride(q, 1), _stride(q, 2)
+    a.k, a.k_bs, a.k_ss, a.k_hs = k.data_ptr(), _stride(k, 0), _stride(k, 1), _stride(k, 2)
+    a.v, a.v_bs, a.v_ss, a.v_hs = v.data_ptr(), _stride(v, 0), _stride(v, 1), _stride(v, 2)
+    a.B, a.Sq, a.H, a.Hkv, a.D, a.Skv = B, Sq, H, k.shape[2], D, k.shape[1]
+    a.fp16, a.scale = int(q.dtype == torch.float16), scale
+    if kp is not None and kp.shape[1]:
+        kp, vp = _strided(kp), _strided(vp)
+        a.kp, a.kp_ss, a.kp_hs, a.vp, a.vp_ss, a.vp_hs = (kp.data_ptr(), _stride(kp, 1), _stride(kp, 2), vp.data_ptr(),
+                                                          _stride(vp, 1), _stride(vp, 2))  # fmt: skip
+        a.P = kp.shape[1]
+    a.kv_lens, a.cu_kv, a.key_mask = native.ptr(kv_lens), native.ptr(cu_kv), native.ptr(key_mask)
+    if key_mask is not None:
+        a.mask_bs = key_mask.stride(0)
+    out = torch.empty(B, Sq, H, D, device=q.device, dtype=q.dtype)
+    lse = torch.empty(B, H, Sq, device=q.device, dtype=torch.float32) if return_lse else None
+    if out.numel():
+        a.out, a.lse = out.data_ptr(), native.ptr(lse)
+        lib = native.load()
+        need = lib.tfb_context_attn_work(ctypes.byref(a))
+        if need < 0:
+            native.check(-need, "tfb_context_attn_work")
+        work = torch.empty(need // 4, device=q.device, dtype=torch.float32) if need else None
+        a.work = native.ptr(work)
+        native.check(lib.tfb_context_attn(ctypes.byref(a), native.stream_ptr()), "tfb_context_attn")
+    return (out, lse) if return_lse else out
+
+
+def cross_attention(q, k, v, kv_lens=None, cu_kv=None, key_mask=None, scale=None, return_lse=False):
+    """softmax(scale q k^T) v of q [B, Sq, H, D] over an encoder's states -> [B, Sq, H, D] (and fp32 lse [B, H, Sq]).
+
+    k / v: [B, Skv, Hkv, D], H a multiple of Hkv (query head h reads key head h // (H / Hkv)); of these sample b sees
+    the first `kv_lens[b]` (all by default), without those where `key_mask` [B, Skv] is False. Or, with `cu_kv` [B + 1],
+    packed [T, Hkv, D] (or [1, T, Hkv, D]): sample b sees rows cu_kv[b] .. cu_kv[b + 1] - 1.
+    `kv_lens` / `cu_kv`: lists or CPU tensors (checked, copied to the device) or int32 / int64 device tensors (used in
+    place; out-of-range values are clamped to the tensors). `scale`: 1 / sqrt(D) by default, positive."""
+    if cu_kv is not None:
+        if kv_lens is not None or key_mask is not None:
+            raise ValueError("cross_attention: packed states (cu_kv) exclude kv_lens and key_mask")
+        if k.dim() == 3:
+            k, v = k.unsqueeze(0), v.unsqueeze(0)
+        if k.shape[0] != 1:
+            raise ValueError(f"cross_attention: packed k / v are [T, Hkv, D], got {tuple(k.shape)}")
+    _check(q, k, v, "cross_attention")
+    B, Skv = q.shape[0], k.shape[1]
+    scale = _scale(scale, q.shape[3])
+    if cu_kv is not None:
+        if not torch.is_tensor(cu_kv) or cu_kv.device.type == "cpu":
+            values = [int(x) for x in cu_kv]
+            if any(a > b for a, b in zip(values, values[1:])):
+                raise ValueError(f"cross_attention: cu_kv must not decrease, got {values}")
+        cu_kv = _lengths(cu_kv, B + 1, Skv, q.device, "cu_kv")
+    elif k.shape[0] != B:
+        raise ValueError(f"cross_attention: batch {B} of q against {k.shape[0]} of k / v")
+    if kv_lens is not None:
+        kv_lens = _lengths(kv_lens, B, Skv, q.device, "kv_lens")
+    if key_mask is not None:
+        if key_mask.shape != (B, Skv) or key_mask.dtype != torch.bool:
+            raise ValueError(f"cross_attention: key_mask is bool [{B}, {Skv}], got {key_mask.dtype} {tuple(key_mask.shape)}")
+        native.same_device(q, key_mask)
+        key_mask = key_mask if key_mask.stride(-1) == 1 or Skv == 1 else key_mask.contiguous()
+    if _runs_native(q):
+        return _launch(q, k, v, None, None, kv_lens, cu_kv, key_mask, scale, return_lse)
+    visible = key_mask
+    if cu_kv is not None:
+        cu = [min(max(x, 0), Skv) for x in cu_kv.tolist()]
+        lens = [max(b - a, 0) for a, b in zip(cu, cu[1:])]
+        at = torch.tensor(cu[:-1], device=q.device)[:, None] + torch.arange(max(lens, default=0), device=q.device)
+        visible = torch.arange(at.shape[1], device=q.device) < torch.tensor(lens, device=q.device)[:, None]
+        k, v = (t[0][at.clamp(max=max(Skv - 1, 0))] if Skv else t.new_zeros(B, 0, *t.shape[2:]) for t in (k, v))
+    elif kv_lens is not None:
+        seen = torch.arange(Skv, device=q.device) < kv_lens[:, None]
+        visible = seen if visible is None else visible & seen
+    return context_attention_reference(q, k, v, visible, scale, return_lse, _q_block(q, k.shape[1]))
+
+
+def prefix_attention(q, k_prefix, v_prefix, k, v, kv_lens=None, scale=None, return_lse=False):
+    """Attention of a batch whose samples share a prefix of keys: softmax over the P prefix keys followed by the sample's own.
+
+    q [B, Sq, H, D]; k_prefix / v_prefix [1, P, Hkv, D] (or [P, Hkv, D]), stored once for all samples; k / v
+    [B, S, Hkv, D], of which sample b sees the first `kv_lens[b]` (all by default; P or S may be 0). Equal to `cross_attention` over the
+    concatenation, which is never built. Every query sees every key: causal order among the own tokens is not applied.
+    With few queries per sample (single tokens) the prefix is read once for the whole batch instead of once per sample."""
+    if k_prefix.dim() == 3:
+        k_prefix, v_prefix = k_prefix.unsqueeze(0), v_prefix.unsqueeze(0)
+    _check(q, k, v, "prefix_attention")
+    _check(q, k_prefix, v_prefix, "prefix_attention (prefix)")
+    if k_prefix.shape[0] != 1 or k_prefix.shape[2] != k.shape[2]:
+        raise ValueError(f"prefix_attention: the shared prefix is [1, P, {k.shape[2]}, {k.shape[3]}], got {tuple(k_prefix.shape)}")
+    B, S = q.shape[0], k.shape[1]
+    if k.shape[0] != B:
+        raise ValueError(f"prefix_attention: batch {B} of q against {k.shape[0]} of k / v")
+    scale = _scale(scale, q.shape[3])
+    if kv_lens is not None:
+        kv_lens = _lengths(kv_lens, B, S, q.device, "kv_lens")
+    if _runs_native(q):
+        return _launch(q, k, v, k_prefix, v_prefix, kv_lens, None, None, scale, return_lse)
+    visible = None
+    if kv_lens is not None:
+        P = k_prefix.shape[1]
+        visible = torch.arange(P + S, device=q.device) < P + kv_lens.clamp(0, S)[:, None]
+    k, v = (torch.cat([a.expand(B, -1, -1, -1), b], dim=1) for a, b in ((k_prefix, k), (v_prefix, v)))
+    return context_attention_reference(q, k, v, visible, scale, return_lse, _q_block(q, k.shape[1]))
+
+
+__all__ = ["cross_attention", "prefix_attention", "context_attention_reference"]

@@ -1130,6 +1130,91 @@ def rmsnorm_gate_residual(res, y, weight=None, gate=None, eps=1e-6, tanh_gate=Tr
     return out.view(res.shape)
 
 
+def _row_table(t, B, rows, C):
+    """fp32 modulation table of 1, B or `rows` rows of C -> (tensor, row stride, rows of the activations per table row).
+    Slices of a wider table are used in place (their row stride is kept)."""
+    t = t.float()
+    n = t.numel() // C
+    if t.shape[-1] != C or n not in (1, B, rows):
+        raise ValueError(f"a modulation table of shape {tuple(t.shape)} does not fit {B} samples / {rows} rows of {C}")
+    lead = [(m, st) for m, st in zip(t.shape[:-1], t.stride()[:-1]) if m > 1]
+    if len(lead) > 1 and all(lead[i][1] == lead[i + 1][0] * lead[i + 1][1] for i in range(len(lead) - 1)):
+        lead = [(n, lead[-1][1])]
+    ld = lead[0][1] if lead else 0
+    if len(lead) > 1 or ld % 4 or t.stride(-1) != 1 or t.data_ptr() % 16:
+        t, ld = t.clone(memory_format=torch.contiguous_format), C
+    return t, ld, max(1, rows // n)
+
+
+def rmsnorm_gate_residual_modulate(res, y, weight=None, gate=None, next_weight=None, shift=None, scale=None, eps=1e-6,
+                                   tanh_gate=True, post_norm=True):  # fmt: skip
+    """The end of one sub-layer and the start of the next in one pass -> (x, h):
+
+        x = res + g * (weight * rmsnorm(y))                  g = tanh(gate), or gate with tanh_gate=False
+        h = next_weight * rmsnorm(x) * (1 + scale) + shift
+
+    i.e. `rmsnorm_gate_residual` followed by `rmsnorm_modulate`; h is taken from x as it is stored. With post_norm=False
+    y enters without a norm (and without `weight`). res / y: [..., C] bf16, fp16 or fp32 on CUDA with C % 8 == 0 up to 8192, others
+    take the two reference steps; weights [C]; gate / shift / scale: [1 | B, 1, C] or [B, S, C]."""
+    if res.shape != y.shape or res.dtype != y.dtype:
+        raise ValueError(f"residual {res.dtype} {tuple(res.shape)} and branch {y.dtype} {tuple(y.shape)} must match")
+    if not post_norm and weight is not None:
+        raise ValueError("post_norm=False takes no weight for the norm of y")
+    C = res.shape[-1]
+    for w in (weight, next_weight):
+        if w is not None and w.shape != (C,):
+            raise ValueError(f"a norm weight has shape ({C},), got {tuple(w.shape)}")
+    native.same_device(res, y, weight, gate, next_weight, shift, scale)
+    if not _native(res) or res.dtype not in _SNORM_TYPES or C % 8 or C > 8192:
+        n = _rms(y, weight, eps) if post_norm else y.float()
+        if gate is not None:
+            n = (gate.float().tanh() if tanh_gate else gate.float()) * n
+        x = (res.float() + n).to(res.dtype)
+        h = _rms(x, next_weight, eps)
+        if scale is not None:
+            h = h * (1.0 + scale.float())
+        if shift is not None:
+            h = h + shift.float()
+        return x, h.to(res.dtype)
+    if res.device.index != torch.cuda.current_device():
+        with torch.cuda.device(res.device):
+            return rmsnorm_gate_residual_modulate(res, y, weight, gate, next_weight, shift, scale, eps, tanh_gate, post_norm)
+    rows = res.numel() // C if C else 0
+    x, h = (torch.empty(res.shape, device=res.device, dtype=res.dtype) for _ in range(2))
+    if rows == 0:
+        return x, h
+
+    def matrix(t):
+        t = t.reshape(rows, C)
+        ok = (t.stride(1) == 1 or C == 1) and t.data_ptr() % 16 == 0 and (rows == 1 or t.stride(0) * t.element_size() % 16 == 0)
+        t = t if ok else t.clone(memory_format=torch.contiguous_format)
+        return t, t.stride(0) if rows > 1 else C
+
+    r2, ldr = matrix(res)
+    y2, ldy = matrix(y)
+    weights = [w for w in (weight, next_weight) if w is not None]
+    w_f32 = any(w.dtype != res.dtype for w in weights)
+
+    def vector(w):
+        if w is None:
+            return None
+        w = (w.float() if w_f32 else w).contiguous()
+        return w if w.data_ptr() % 16 == 0 else w.clone()
+
+    w1, w2 = vector(weight), vector(next_weight)
+    B = res.shape[0] if res.dim() > 2 else 1
+    g, sh, sc = ((None, 0, 1) if t is None else _row_table(t, B, rows, C) for t in (gate, shift, scale))
+    code = native.load().tfb_sandwich_norm(
+        r2.data_ptr(), ldr, y2.data_ptr(), ldy, x.data_ptr(), h.data_ptr(), rows, C, float(eps), _SNORM_TYPES[res.dtype],
+        int(w_f32), native.ptr(w1), native.ptr(w2), native.ptr(g[0]), g[1], g[2], native.ptr(sh[0]), sh[1], sh[2],
+        native.ptr(sc[0]), sc[1], sc[2], int(post_norm), int(tanh_gate), native.stream_ptr())  # fmt: skip
+    native.check(code, "tfb_sandwich_norm")
+    return x, h
+
+
+_SNORM_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
 def headnorm_rope_(q, weight_q, cos=None, sin=None, eps=1e-6, k=None, weight_k=None):
     """In place on q (and k): per-head RMSNorm over the last dim, then interleaved-pair RoPE.
     q / k: [B, S, H, D] views (possibly slices of one fused buffer); cos / sin: fp32 [B*S, D/2]."""

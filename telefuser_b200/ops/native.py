@@ -138,9 +138,15 @@ def _declare(lib) -> None:
                              c_int, c_int, c_void_p, c_int, c_void_p],
         "tfb_slab_reduce": [c_void_p, c_int, c_long, c_int, c_long, c_void_p, c_void_p, c_long, c_void_p, c_long, c_int,
                             c_long, c_void_p, c_int, c_long, c_long, c_void_p],
+        "tfb_context_attn": [c_void_p, c_void_p],
+        "tfb_sandwich_norm": [c_void_p, c_long, c_void_p, c_long, c_void_p, c_void_p, c_long, c_int, c_float, c_int, c_int,
+                              c_void_p, c_void_p, c_void_p, c_long, c_long, c_void_p, c_long, c_long, c_void_p, c_long,
+                              c_long, c_int, c_int, c_void_p],
         "tfb_attn_fwd_peer": [c_void_p, c_long, c_long, c_void_p, c_long, c_long, c_void_p, c_long, c_long, c_void_p,
                               c_int, c_int, c_int, c_long, c_long, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p],
     }  # fmt: skip
+    lib.tfb_context_attn_work.restype = c_long
+    lib.tfb_context_attn_work.argtypes = [c_void_p]
     for name, args in table.items():
         fn = getattr(lib, name)
         fn.restype = c_int
