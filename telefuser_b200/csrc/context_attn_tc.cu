@@ -3,18 +3,21 @@
 //
 // Persistent: one CTA per SM walks over work items (sample, head group, pair of 128-row query tiles, key slice). A tile's
 // rows are (token, head) pairs of one key head where the head group is a power of two, so grouped heads share every K / V
-// tile; otherwise a tile is 128 tokens of one head. 384 threads:
-//   warps 0..3  softmax group 0 (query tile 0; TMEM lane == row)       warp 8   TMA loader
-//   warps 4..7  softmax group 1 (query tile 1)                         warp 9   tcgen05.mma issuer, TMEM owner
-//   warp 10     tail / mask warp: clears the V rows that nobody may see before the P.V product reads them (a product
-//               with infinities or NaN there would spread through P = 0) and turns the key mask into bit words
-//   warp 11     only donates registers
+// tile; otherwise a tile is 128 tokens of one head. 512 threads:
+//   warp 0   TMA loader                                   warps 4..7    softmax group 0 (query tile 0; TMEM lane == row)
+//   warp 1   tcgen05.mma issuer, TMEM owner               warps 8..11   softmax group 1 (query tile 1)
+//   warp 3   decodes the work items into a ring           warps 12..15  output of finished tiles
+//   warp 2   tail / mask warp: clears the V rows that nobody may see before the P.V product reads them (a product with
+//            infinities or NaN there would spread through P = 0) and turns the key mask into bit words
 // TMEM (512 columns): S0 | S1 | O0 | O1. P overwrites the first 64 columns of its S tile and enters P.V from TMEM.
 // Encoder states are short (a prompt is 1 .. 4 blocks of 128 keys), so the ends of an item count: the issuer starts the
-// next item's Q.K^T of a tile right behind the last P.V of that tile, the loader is a whole item ahead, and a softmax
-// group writes its output (through shared memory and TMA stores that clip at the tensor's edge) while the other group
-// and the tensor core work on. The last block of a sample is as narrow as its keys need: 32-column steps in Q.K^T, the
-// exponentials and P.V.
+// next item's Q.K^T of a tile right behind the last P.V of that tile, the loader is a whole item ahead, and normalising
+// and writing a tile is the output warps' business (shared memory, then TMA stores that clip at the tensor's edge) while the
+// softmax groups go on with the next item. The last block of a sample is as narrow as its keys need: 32-column steps in
+// Q.K^T, the exponentials and P.V.
+// The issuer is the warp that everything waits for: a P.V + Q.K^T pair takes the tensor core 1024 clk, and its 16
+// instructions took 1500 clk to issue while descriptors sat in per-lane registers. Its values are warp-uniform by
+// construction (items come through shuffles) and one elected lane issues.
 //
 // The row maximum that exp2 uses is only raised when it grew by more than 2^8. P is rounded to the inputs' type for the
 // product (at most 2^8, sum in fp32).
@@ -28,10 +31,16 @@ constexpr int CT_TILE = 128 * 128 * 2;  // 32 KB: two boxes of [128 rows][64 cha
 constexpr int CT_BOX = 128 * 64 * 2;
 constexpr int CT_Q_OFF = 0;
 constexpr int CT_KV_OFF = 2 * CT_TILE;               // K ring of 2, then V ring of 2
-constexpr int CT_OUT_OFF = CT_KV_OFF + 4 * CT_TILE;  // 8 warps x 2 buffers x [32 rows][32 channels]
-constexpr int CT_BAR_OFF = CT_OUT_OFF + 8 * 4096;
-constexpr int CT_SMEM_BYTES = CT_BAR_OFF + 256 + 1024;
+constexpr int CT_OUT_OFF = CT_KV_OFF + 4 * CT_TILE;  // 4 output warps x 2 boxes of [32 rows][64 channels]
+constexpr int CT_ML_OFF = CT_OUT_OFF + 4 * 8192;     // [2 tiles][128 rows] of (maximum, sum)
+constexpr int CT_ITEMS = 4;                          // ring of decoded items
+constexpr int CT_ITEM_OFF = CT_ML_OFF + 2 * 128 * 8;
+constexpr int CT_BAR_OFF = CT_ITEM_OFF + CT_ITEMS * 32;
+constexpr int CT_N_BARS = 21 + 2 * CT_ITEMS;
+constexpr int CT_ALIGN_SLACK = 512;  // dynamic shared memory starts on 1 KB here; the kernel checks that the tiles fit
+constexpr int CT_SMEM_BYTES = CT_BAR_OFF + (CT_N_BARS + 1) * 8 + 64 + CT_ALIGN_SLACK;
 static_assert(CT_SMEM_BYTES <= 227 * 1024, "shared memory of one CTA");
+constexpr int CT_ITEM_READERS = 3 + 8 + 4;  // loader, issuer and tail warp, softmax warps, output warps
 constexpr float CT_RESCALE_THRESHOLD = 8.0f;
 
 struct CtxTcParams {
@@ -46,10 +55,11 @@ struct CtxTcParams {
 };
 
 struct CtxItem {
-  int b, hg, qp, split;
+  int b;           // -1: no more items
+  int hg, qp, split;
   int first, len;  // the sample's own keys
-  int j0, j1;      // key blocks [j0, j1) of prefix blocks followed by own blocks
-  bool two;        // the second query tile has rows
+  int j0, nb;      // key blocks [j0, j0 + nb) of prefix blocks followed by own blocks
+  __device__ __forceinline__ bool two(const CtxTcParams& p) const { return (qp * 2 + 1) * p.tok < p.c.Sq; }
 };
 
 __device__ __forceinline__ CtxItem ctx_item(const CtxTcParams& p, int i) {
@@ -63,26 +73,147 @@ __device__ __forceinline__ CtxItem ctx_item(const CtxTcParams& p, int i) {
   ctx_sample_range(p.c, t.b, t.first, t.len);
   const long nb = p.n_prefix + ((t.len + 127) >> 7);
   t.j0 = static_cast<int>(nb * t.split / p.c.ns);
-  t.j1 = static_cast<int>(nb * (t.split + 1) / p.c.ns);
-  t.two = (t.qp * 2 + 1) * p.tok < p.c.Sq;
+  t.nb = static_cast<int>(nb * (t.split + 1) / p.c.ns) - t.j0;
   return t;
 }
-// Visible keys of block j at most 128 (before the mask).
-__device__ __forceinline__ int ctx_block_keys(const CtxTcParams& p, const CtxItem& t, int j) {
-  return min(128, j < p.n_prefix ? p.c.P - j * 128 : t.len - (j - p.n_prefix) * 128);
+// Visible keys of block j, at most 128 (before the mask).
+__device__ __forceinline__ int ctx_block_keys(const CtxTcParams& p, int j, int len) {
+  return min(128, j < p.n_prefix ? p.c.P - j * 128 : len - (j - p.n_prefix) * 128);
 }
-// The next item of this CTA that has keys.
-__device__ __forceinline__ bool ctx_next(const CtxTcParams& p, int& i, CtxItem& t) {
-  while (i < p.n_items) {
-    t = ctx_item(p, i);
-    i += gridDim.x;
-    if (t.j1 > t.j0) return true;
+
+// The ring of decoded items as one reader warp sees it.
+struct CtxItems {
+  const int4* ring;
+  uint64_t *full, *empty;
+  int n;
+  // Whole warp; every field comes out warp-uniform. False at the end of the work or on an abort.
+  __device__ __forceinline__ bool next(CtxItem& t, const AbortCtx& ctx, int site) {
+    const int slot = n % CT_ITEMS;
+    if (!mbar_wait_warp(&full[slot], (n / CT_ITEMS) & 1, ctx, site)) return false;
+    ++n;
+    const int4 a = ring[slot * 2], b = ring[slot * 2 + 1];
+    __syncwarp();
+    if (lane_id() == 0) mbar_arrive(&empty[slot]);
+    t.b = __shfl_sync(0xffffffffu, a.x, 0), t.hg = __shfl_sync(0xffffffffu, a.y, 0);
+    t.qp = __shfl_sync(0xffffffffu, a.z, 0), t.split = __shfl_sync(0xffffffffu, a.w, 0);
+    t.first = __shfl_sync(0xffffffffu, b.x, 0), t.len = __shfl_sync(0xffffffffu, b.y, 0);
+    t.j0 = __shfl_sync(0xffffffffu, b.z, 0), t.nb = __shfl_sync(0xffffffffu, b.w, 0);
+    return t.b >= 0;
   }
-  return false;
+};
+
+// The part that both score tile forms share: raises the row maximum when it grew by more than 2^8 (or at the first tile),
+// taking the accumulator and the sum along. All MMAs issued before this tile's scores have completed, so O is stable.
+template <int DK>
+__device__ __forceinline__ void ctx_new_max(uint32_t tmem_o, float m_new, bool first, float& m_used, float& l) {
+  if (first) {
+    m_used = m_new;
+  } else if (__any_sync(0xffffffffu, (m_new - m_used) > CT_RESCALE_THRESHOLD)) {
+    const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_used - m_new);
+    m_used = m_new;
+    l *= alpha;
+#pragma unroll 1
+    for (int c = 0; c < DK / 32; ++c) {
+      uint32_t o[32];
+      tmem_ld_32x32(tmem_o + c * 32, o);
+      tmem_ld_wait();
+#pragma unroll
+      for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+      tmem_st_32x32(tmem_o + c * 32, o);
+    }
+  }
+}
+
+// p = 2^(s scale - m) of 32 columns, added up in ps and packed into TMEM: packed fp32x2 FMAs and row sums.
+template <bool FP16>
+__device__ __forceinline__ void ctx_exp32(const uint32_t (&s)[32], uint32_t tmem_p, uint64_t scale2, uint64_t negm2,
+                                          uint64_t (&ps)[4]) {
+  uint32_t pk[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const uint64_t x2 = f2_fma(f2_pack(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), scale2, negm2);
+    float x0, x1;
+    f2_unpack(x2, x0, x1);
+    const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+    ps[k & 3] = f2_add(ps[k & 3], f2_pack(p0, p1));
+    pk[k] = ctx_pack2<FP16>(p0, p1);
+  }
+  tmem_st_32x16(tmem_p, pk);
+}
+__device__ __forceinline__ float ctx_sum(const uint64_t (&ps)[4]) {
+  float a0, a1, b0, b1;
+  f2_unpack(f2_add(ps[0], ps[1]), a0, a1);
+  f2_unpack(f2_add(ps[2], ps[3]), b0, b1);
+  return (a0 + a1) + (b0 + b1);
+}
+
+// A full 128 x 128 score tile: scores from TMEM to registers, maximum, exponentials, P back over the scores.
+template <bool FP16, int DK>
+__device__ __forceinline__ void ctx_softmax_full(uint32_t tmem_s, uint32_t tmem_o, float scale_log2, bool first, float& m_used,
+                                                 float& l) {
+  uint32_t s[4][32];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) tmem_ld_32x32(tmem_s + c * 32, s[c]);
+  tmem_ld_wait();
+  // Row maximum: 8 independent chains of 3-input max.
+  float mx8[8];
+#pragma unroll
+  for (int a = 0; a < 8; ++a) mx8[a] = __uint_as_float(s[a >> 1][a & 1]);
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int e = 2; e < 32; e += 4) {
+      mx8[c * 2] = fmax3(mx8[c * 2], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+      if (e + 3 < 32)
+        mx8[c * 2 + 1] = fmax3(mx8[c * 2 + 1], __uint_as_float(s[c][e + 2]), __uint_as_float(s[c][e + 3]));
+    }
+  const float mx = fmax3(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]));
+  ctx_new_max<DK>(tmem_o, fmaxf(m_used, mx * scale_log2), first, m_used, l);
+  const float neg = m_used == -INFINITY ? 0.f : -m_used;
+  uint64_t ps[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    ctx_exp32<FP16>(s[c], tmem_s + c * 16, f2_pack(scale_log2, scale_log2), f2_pack(neg, neg), ps);
+  l += ctx_sum(ps);
+}
+
+// A narrow tile (32-column steps) or one with hidden keys (their bits in `words` are clear): 32 columns at a time, the
+// scores read from TMEM once for the maximum and once for the exponentials, which keeps the registers of the full form
+// to itself. P of step c overwrites columns that steps <= c have read.
+template <bool FP16, int DK, bool MASK>
+__device__ __forceinline__ void ctx_softmax_part(uint32_t tmem_s, uint32_t tmem_o, float scale_log2, int keys,
+                                                 volatile const uint32_t* words, bool first, float& m_used, float& l) {
+  const int chunks = (keys + 31) >> 5;
+  uint32_t s[32];
+  auto load = [&](int c) {
+    tmem_ld_32x32(tmem_s + c * 32, s);
+    const int left = keys - c * 32;
+    const uint32_t vis = (MASK ? words[c] : 0xffffffffu) & (left >= 32 ? 0xffffffffu : (1u << left) - 1u);
+    tmem_ld_wait();
+#pragma unroll
+    for (int e = 0; e < 32; ++e)
+      if (!((vis >> e) & 1)) s[e] = 0xff800000u;  // -inf
+  };
+  float mx = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < chunks; ++c) {
+    load(c);
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) mx = fmax3(mx, __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+  }
+  ctx_new_max<DK>(tmem_o, fmaxf(m_used, mx * scale_log2), first, m_used, l);
+  const float neg = m_used == -INFINITY ? 0.f : -m_used;
+  uint64_t ps[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll 1
+  for (int c = 0; c < chunks; ++c) {
+    load(c);
+    ctx_exp32<FP16>(s, tmem_s + c * 16, f2_pack(scale_log2, scale_log2), f2_pack(neg, neg), ps);
+  }
+  l += ctx_sum(ps);
 }
 
 template <bool FP16, int DK, bool MASK>
-__global__ void __launch_bounds__(384, 1)
+__global__ void __launch_bounds__(512, 1)
     ctx_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmKp,
                   const __grid_constant__ CUtensorMap tmVp, const __grid_constant__ CUtensorMap tmO,
@@ -91,22 +222,30 @@ __global__ void __launch_bounds__(384, 1)
   constexpr uint32_t LOAD_BYTES = NBOX * CT_BOX;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  if (smem - smem_raw > CT_ALIGN_SLACK) {  // same verdict in every thread
+    if (threadIdx.x == 0 && p.c.status) atomicCAS(p.c.status, 0, TFB_ERR_TOO_LARGE | (62 << 8));
+    return;
+  }
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + CT_BAR_OFF);
-  uint64_t* q_full = bars + 0;    // [2] per query tile
-  uint64_t* q_empty = bars + 2;   // [2]
-  uint64_t* k_full = bars + 4;    // [2] per ring slot
-  uint64_t* k_empty = bars + 6;   // [2]
-  uint64_t* v_full = bars + 8;    // [2]
-  uint64_t* v_empty = bars + 10;  // [2]
-  uint64_t* v_ready = bars + 12;  // [2] hidden rows cleared, mask words written
-  uint64_t* s_full = bars + 14;   // [2] per query tile
-  uint64_t* p_ready = bars + 16;  // [2]
-  uint64_t* o_final = bars + 18;  // [2]
-  uint32_t* words = reinterpret_cast<uint32_t*>(bars + 20);  // [2 slots][4]
+  uint64_t* q_full = bars + 0;     // [2] per query tile
+  uint64_t* q_empty = bars + 2;    // [2]
+  uint64_t* kv_full = bars + 4;    // [2] stage g & 1: V of key block g and K of block g + 1
+  uint64_t* kv_ready = bars + 6;   // [2] ... with the hidden V rows cleared and the mask words of block g written
+  uint64_t* kv_empty = bars + 8;   // [2]
+  uint64_t* s_full = bars + 10;    // [2] per query tile
+  uint64_t* p_ready = bars + 12;   // [2]
+  uint64_t* o_final = bars + 14;   // [2] the tile's last P.V is done
+  uint64_t* l_full = bars + 16;    // [2] the tile's maxima and sums are in shared memory
+  uint64_t* o_empty = bars + 18;   // [2] accumulator, maxima and sums have been read
+  uint64_t* k_first = bars + 20;   // K of block 0
+  uint64_t* i_full = bars + 21;    // [CT_ITEMS]
+  uint64_t* i_empty = i_full + CT_ITEMS;
+  uint32_t* words = reinterpret_cast<uint32_t*>(bars + ((CT_N_BARS + 1) & ~1));  // [2 slots][4]
   uint32_t* tmem_slot = words + 8;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float2* ml = reinterpret_cast<float2*>(smem + CT_ML_OFF);
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
   AbortCtx ctx{abort_flag, p.c.status};
 
@@ -114,19 +253,24 @@ __global__ void __launch_bounds__(384, 1)
     for (int s = 0; s < 2; ++s) {
       mbar_init(&q_full[s], 1);
       mbar_init(&q_empty[s], 1);
-      mbar_init(&k_full[s], 1);
-      mbar_init(&k_empty[s], 1);
-      mbar_init(&v_full[s], 1);
-      mbar_init(&v_empty[s], 1);
-      mbar_init(&v_ready[s], 32);
+      mbar_init(&kv_full[s], 1);
+      mbar_init(&kv_ready[s], 1);
+      mbar_init(&kv_empty[s], 1);
       mbar_init(&s_full[s], 1);
       mbar_init(&p_ready[s], 128);
       mbar_init(&o_final[s], 1);
+      mbar_init(&l_full[s], 128);
+      mbar_init(&o_empty[s], 4);
+    }
+    mbar_init(k_first, 1);
+    for (int s = 0; s < CT_ITEMS; ++s) {
+      mbar_init(&i_full[s], 1);
+      mbar_init(&i_empty[s], CT_ITEM_READERS);
     }
     *abort_flag = 0;
     mbar_fence_init();
   }
-  if (warp == 9) {
+  if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -134,362 +278,368 @@ __global__ void __launch_bounds__(384, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  CtxItems items{reinterpret_cast<const int4*>(smem + CT_ITEM_OFF), i_full, i_empty, 0};
+  CtxItem t;
 
-  // Registers move only inside the launch allocation: 256 x 216 + 128 x 72 = 384 x 168.
-  static_assert(256 * 216 + 128 * 72 <= 384 * 168, "setmaxnreg split");
-  if (warp >= 8) {
+  // Registers move only inside the launch allocation of 512 x 128; these shares spill least (16 bytes).
+  static_assert(256 * 176 + 128 * 88 + 128 * 72 <= 512 * 128, "setmaxnreg split");
+  if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (warp == 8) {
-      // ------------------------------ TMA loader ------------------------------
-      if (lane == 0) {
-        tma_prefetch_desc(&tmQ);
-        tma_prefetch_desc(&tmK);
-        tma_prefetch_desc(&tmV);
-        CtxItem t;
-        int i = blockIdx.x, g = 0;
-        int nq[2] = {0, 0};
-        bool ok = true;
-        while (ok && ctx_next(p, i, t)) {
-          const int hk = t.hg * p.pack / (p.c.H / p.c.Hkv);
-          for (int j = t.j0; j < t.j1 && ok; ++j, ++g) {
-            const int slot = g & 1;
-            const uint32_t ph = (g >> 1) & 1;
-            const bool pre = j < p.n_prefix;
-            const int row = pre ? j * 128 : t.first + (j - p.n_prefix) * 128;
-            if (!(ok = mbar_wait(&k_empty[slot], ph ^ 1, ctx, 40))) break;
-            uint8_t* dst = smem + CT_KV_OFF + slot * CT_TILE;
-            const CUtensorMap* tm = pre ? &tmKp : &tmK;
-            mbar_expect_tx(&k_full[slot], LOAD_BYTES);
-            for (int x = 0; x < NBOX; ++x)
-              tma_load_4d(dst + x * CT_BOX, tm, &k_full[slot], x * 64, hk, row, pre ? 0 : t.b * p.bmul);
-            if (j == t.j0) {
-              for (int st = 0; st < (t.two ? 2 : 1); ++st) {
-                if (!(ok = mbar_wait(&q_empty[st], (nq[st] & 1) ^ 1, ctx, 41))) break;
-                ++nq[st];
-                mbar_expect_tx(&q_full[st], LOAD_BYTES);
-                for (int x = 0; x < NBOX; ++x)
-                  tma_load_4d(smem + CT_Q_OFF + st * CT_TILE + x * CT_BOX, &tmQ, &q_full[st], x * 64, t.hg * p.pack,
-                              (t.qp * 2 + st) * p.tok, t.b);
-              }
-              if (!ok) break;
-            }
-            if (!(ok = mbar_wait(&v_empty[slot], ph ^ 1, ctx, 42))) break;
-            dst = smem + CT_KV_OFF + (2 + slot) * CT_TILE;
-            tm = pre ? &tmVp : &tmV;
-            mbar_expect_tx(&v_full[slot], LOAD_BYTES);
-            for (int x = 0; x < NBOX; ++x)
-              tma_load_4d(dst + x * CT_BOX, tm, &v_full[slot], x * 64, hk, row, pre ? 0 : t.b * p.bmul);
-          }
-        }
-      }
-      __syncwarp();
-    } else if (warp == 9) {
-      // ------------------------------ MMA issuer ------------------------------
-      constexpr uint32_t FMT = FP16 ? 0 : 1;
-      constexpr uint32_t idesc_pv = make_idesc(128, DK, FMT, FMT, 0, 1);  // B (= V) is MN-major
-      CtxItem t, nt;
-      int i = blockIdx.x, g = 0;
-      int nq[2] = {0, 0}, np[2] = {0, 0};
-      bool ok = true;
-      // Q.K^T of key block j into S of query tile st; `last`: no further block of this item reads the Q tile
-      auto issue_qk = [&](int st, const CtxItem& it, int j, int gg, bool last) {
-        const uint32_t idesc = make_idesc(128, (ctx_block_keys(p, it, j) + 31) & ~31, FMT, FMT, 0, 0);
-        const uint32_t q_addr = smem_u32(smem + CT_Q_OFF + st * CT_TILE);
-        const uint32_t k_addr = smem_u32(smem + CT_KV_OFF + (gg & 1) * CT_TILE);
-#pragma unroll
-        for (int kk = 0; kk < DK / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * CT_BOX + (kk & 3) * 32;
-          umma_f16_ss(tmem_base + st * 128, make_desc_k_sw128(q_addr + off), make_desc_k_sw128(k_addr + off), idesc,
-                      kk ? 1u : 0u);
-        }
-        umma_commit(&s_full[st]);
-        if (last) umma_commit(&q_empty[st]);
-      };
-      auto prime = [&](int st, const CtxItem& it, int gg) {
-        if (!mbar_wait_warp(&q_full[st], nq[st] & 1, ctx, 43)) return false;
-        ++nq[st];
-        if (!mbar_wait_warp(&k_full[gg & 1], (gg >> 1) & 1, ctx, 44)) return false;
-        tc_fence_after();
-        if (lane == 0) issue_qk(st, it, it.j0, gg, it.j1 - it.j0 == 1);
-        __syncwarp();
-        return true;
-      };
-      bool have = ctx_next(p, i, t);
-      if (have) {
-        ok = prime(0, t, 0) && (!t.two || prime(1, t, 0));
-        if (ok && lane == 0) umma_commit(&k_empty[0]);
-        __syncwarp();
-      }
-      while (have && ok) {
-        const int nb = t.j1 - t.j0, gn = g + nb;
-        const bool have_next = ctx_next(p, i, nt);
-        for (int n = 0; n < nb && ok; ++n) {
-          const int gv = g + n;
-          const bool more = n + 1 < nb;
-          const int steps = ((ctx_block_keys(p, t, t.j0 + n) + 31) >> 5) * 2;
-          ok = mbar_wait_warp(&v_full[gv & 1], (gv >> 1) & 1, ctx, 52) &&
-               mbar_wait_warp(&v_ready[gv & 1], (gv >> 1) & 1, ctx, 45) &&
-               (!more || mbar_wait_warp(&k_full[(gv + 1) & 1], ((gv + 1) >> 1) & 1, ctx, 46));
-          for (int st = 0; st < (t.two ? 2 : 1) && ok; ++st) {
-            if (!(ok = mbar_wait_warp(&p_ready[st], np[st] & 1, ctx, 47))) break;
-            ++np[st];
-            tc_fence_after();
-            if (lane == 0) {
-              const uint32_t v_addr = smem_u32(smem + CT_KV_OFF + (2 + (gv & 1)) * CT_TILE);
-              const uint32_t o_tmem = tmem_base + 256 + st * 128, p_tmem = tmem_base + st * 128;
-              for (int kk = 0; kk < steps; ++kk)
-                umma_f16_ts(o_tmem, p_tmem + kk * 8, make_desc_mn_sw128(v_addr + kk * 2048, CT_BOX), idesc_pv,
-                            (n | kk) ? 1u : 0u);
-              if (more)
-                issue_qk(st, t, t.j0 + n + 1, gv + 1, n + 2 == nb);
-              else
-                umma_commit(&o_final[st]);
-            }
-            __syncwarp();
-            if (!more && have_next && (st == 0 || nt.two)) ok = prime(st, nt, gn);
-          }
-          if (ok && lane == 0) {
-            umma_commit(&v_empty[gv & 1]);
-            if (more) umma_commit(&k_empty[(gv + 1) & 1]);
-          }
-          __syncwarp();
-        }
-        if (ok && have_next) {
-          if (nt.two && !t.two) ok = prime(1, nt, gn);
-          if (ok && lane == 0) umma_commit(&k_empty[gn & 1]);
-          __syncwarp();
-        }
-        have = have_next;
-        t = nt;
-        g = gn;
-      }
-    } else if (warp == 10) {
-      // ------------------------------ tail / mask warp ------------------------------
-      CtxItem t;
-      int i = blockIdx.x, g = 0;
-      bool ok = true;
-      while (ok && ctx_next(p, i, t)) {
-        for (int j = t.j0; j < t.j1; ++j, ++g) {
-          const int slot = g & 1;
-          const int keys = ctx_block_keys(p, t, j), cols = (keys + 31) & ~31;
-          uint32_t w[4];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int key = x * 32 + lane;
-            bool vis = key < keys;
-            if (MASK && vis)
-              vis = __ldg(p.c.key_mask + static_cast<long>(t.b) * p.c.mask_bs + (j - p.n_prefix) * 128 + key) != 0;
-            w[x] = __ballot_sync(0xffffffffu, vis);
-          }
-          if (!(ok = mbar_wait_warp(&v_full[slot], (g >> 1) & 1, ctx, 48))) break;
-          bool wrote = false;
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            if (x * 32 < cols && w[x] != 0xffffffffu) {
-              wrote = true;
-              if (!((w[x] >> lane) & 1)) {
-                uint4* row = reinterpret_cast<uint4*>(smem + CT_KV_OFF + (2 + slot) * CT_TILE + (x * 32 + lane) * 128);
-#pragma unroll
-                for (int y = 0; y < NBOX; ++y)
-#pragma unroll
-                  for (int e = 0; e < 8; ++e) row[y * (CT_BOX / 16) + e] = make_uint4(0, 0, 0, 0);
-              }
-            }
-            if (MASK && lane == x) words[slot * 4 + x] = w[x];
-          }
-          if (wrote) fence_proxy_async_smem();
-          mbar_arrive(&v_ready[slot]);
-        }
-      }
-    }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    // ------------------------------ softmax groups ------------------------------
-    const int st = warp >> 2;
-    const int row = (warp & 3) * 32 + lane;
-    const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t tmem_s = tmem_base + lane_addr + st * 128;
-    const uint32_t tmem_o = tmem_base + lane_addr + 256 + st * 128;
-    uint8_t* stage = smem + CT_OUT_OFF + warp * 4096;
+    // ------------------------------ output warps ------------------------------
+    const int wq = warp & 3;
+    const int row = wq * 32 + lane;
+    const uint32_t lane_addr = static_cast<uint32_t>(wq * 32) << 16;
+    uint8_t* stage = smem + CT_OUT_OFF + wq * 8192;
     const int row_tok = row / p.pack, row_head = row % p.pack;
-    int ns = 0, no = 0, g = 0, nout = 0;  // score tiles, items, key blocks and output steps so far
+    uint32_t o_phase = 0;  // bit per query tile
     bool ok = true;
-    for (int i = blockIdx.x; i < p.n_items && ok; i += gridDim.x) {
-      const CtxItem t = ctx_item(p, i);
-      const int nb = t.j1 - t.j0;
-      if (st && !t.two) {
-        g += nb;
-        continue;
-      }
-      float m_used = -INFINITY, l = 0.f;
-      for (int n = 0; n < nb; ++n, ++g) {
-        uint32_t w[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-        const int keys = ctx_block_keys(p, t, t.j0 + n);
-        const int chunks = (keys + 31) >> 5;
-        if (!(ok = mbar_wait_warp(&s_full[st], ns & 1, ctx, 50))) break;
-        ++ns;
-        tc_fence_after();
-        if (MASK) {
-          // behind s_full: the scores of block g exist only once v_ready of block g - 1 has completed, so the parity of
-          // block g cannot be mistaken for that of block g - 4 by a group that skipped items
-          if (!(ok = mbar_wait_warp(&v_ready[g & 1], (g >> 1) & 1, ctx, 49))) break;
-#pragma unroll
-          for (int x = 0; x < 4; ++x) w[x] = *reinterpret_cast<volatile uint32_t*>(&words[(g & 1) * 4 + x]);
+    while (ok && items.next(t, ctx, 55)) {
+      for (int st = 0; st < (t.two(p) ? 2 : 1); ++st) {
+        const int tile_tok = (t.qp * 2 + st) * p.tok;
+        const int tok = tile_tok + row_tok, head = t.hg * p.pack + row_head;
+        const bool row_ok = tok < p.c.Sq;
+        const long token = static_cast<long>(t.b) * p.c.Sq + tok;
+        float2 m_l = make_float2(-INFINITY, 0.f);
+        if (t.nb > 0) {
+          if (!(ok = mbar_wait_warp(&l_full[st], (o_phase >> st) & 1, ctx, 56))) break;
+          m_l = ml[st * 128 + row];
         }
-        uint32_t s[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (c < chunks) tmem_ld_32x32(tmem_s + c * 32, s[c]);
-        tmem_ld_wait();
-        if (keys < 128 || (MASK && (w[0] & w[1] & w[2] & w[3]) != 0xffffffffu)) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int left = keys - c * 32;
-            const uint32_t vis = left >= 32 ? w[c] : left <= 0 ? 0u : w[c] & ((1u << left) - 1u);
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!((vis >> e) & 1)) s[c][e] = 0xff800000u;  // -inf
-          }
+        const float inv = m_l.y > 0.f ? 1.f / m_l.y : 0.f;
+        const float lse2 = m_l.y > 0.f ? m_l.x + log2f(m_l.y) : -INFINITY;
+        if (t.nb > 0) {
+          if (!(ok = mbar_wait_warp(&o_final[st], (o_phase >> st) & 1, ctx, 57))) break;
+          o_phase ^= 1u << st;
+          tc_fence_after();
         }
-        // Row maximum: 8 independent chains of 3-input max.
-        float mx8[8];
-#pragma unroll
-        for (int a = 0; a < 8; ++a) mx8[a] = __uint_as_float(s[a >> 1][a & 1]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int e = 2; e < 32; e += 4) {
-            mx8[c * 2] = fmax3(mx8[c * 2], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
-            if (e + 3 < 32)
-              mx8[c * 2 + 1] = fmax3(mx8[c * 2 + 1], __uint_as_float(s[c][e + 2]), __uint_as_float(s[c][e + 3]));
-          }
-        const float mx = fmax3(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]));
-        const float m_new = fmaxf(m_used, mx * p.c.scale_log2);
-        if (n == 0) {
-          m_used = m_new;
-        } else if (__any_sync(0xffffffffu, (m_new - m_used) > CT_RESCALE_THRESHOLD)) {
-          // All MMAs issued before S of this block have completed, so O is stable here.
-          const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_used - m_new);
-          m_used = m_new;
-          l *= alpha;
-#pragma unroll
-          for (int c = 0; c < DK / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld_32x32(tmem_o + c * 32, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st_32x32(tmem_o + c * 32, o);
-          }
-        }
-        // p = 2^(s scale - m): packed fp32x2 FMAs and row sums
-        const uint64_t scale2 = f2_pack(p.c.scale_log2, p.c.scale_log2);
-        const float neg = m_used == -INFINITY ? 0.f : -m_used;
-        const uint64_t negm2 = f2_pack(neg, neg);
-        uint64_t ps[4] = {0ull, 0ull, 0ull, 0ull};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (c < chunks) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const uint64_t x2 =
-                  f2_fma(f2_pack(__uint_as_float(s[c][2 * k]), __uint_as_float(s[c][2 * k + 1])), scale2, negm2);
-              float x0, x1;
-              f2_unpack(x2, x0, x1);
-              const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
-              ps[k & 3] = f2_add(ps[k & 3], f2_pack(p0, p1));
-              pk[k] = ctx_pack2<FP16>(p0, p1);
-            }
-            tmem_st_32x16(tmem_s + c * 16, pk);
-          }
-        }
-        {
-          float a0, a1, b0, b1;
-          f2_unpack(f2_add(ps[0], ps[1]), a0, a1);
-          f2_unpack(f2_add(ps[2], ps[3]), b0, b1);
-          l += (a0 + a1) + (b0 + b1);
-        }
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(&p_ready[st]);
-      }
-      if (!ok) break;
-
-      // ------------------------------ output of one tile ------------------------------
-      const int tile_tok = (t.qp * 2 + st) * p.tok;
-      const int tok = tile_tok + row_tok, head = t.hg * p.pack + row_head;
-      const bool row_ok = tok < p.c.Sq;
-      if (nb > 0) {
-        if (!(ok = mbar_wait_warp(&o_final[st], no & 1, ctx, 51))) break;
-        ++no;
-        tc_fence_after();
-      }
-      const float inv = l > 0.f ? 1.f / l : 0.f;
-      const long token = static_cast<long>(t.b) * p.c.Sq + tok;
-      const float lse2 = l > 0.f ? m_used + log2f(l) : -INFINITY;
-      if (p.c.part_o) {
-        const long at = (static_cast<long>(p.c.slot0 + t.split) * p.c.B * p.c.Sq + token) * p.c.H + head;
-        if (row_ok) p.c.part_lse[at] = lse2;
-        if (nb > 0) {
-#pragma unroll
-          for (int c = 0; c < DK / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld_32x32(tmem_o + c * 32, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              if (row_ok && c * 32 + e < p.c.D)
-                *reinterpret_cast<float4*>(p.c.part_o + at * p.c.D + c * 32 + e) =
-                    make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv,
-                                __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
-          }
-        }
-      } else {
-        if (p.c.lse && row_ok) p.c.lse[(static_cast<long>(t.b) * p.c.H + head) * p.c.Sq + tok] = lse2 * 0.6931471805599453f;
-        // 32 rows x 32 channels per step through this warp's own two buffers (64-byte rows, 64B swizzle)
-#pragma unroll
-        for (int c = 0; c < DK / 32; ++c) {
-          if (c * 32 < p.c.D) {
-            uint32_t o[32];
-            if (nb > 0) {
-              tmem_ld_32x32(tmem_o + c * 32, o);
+        const uint32_t tmem_o = tmem_base + lane_addr + 256 + st * 128;
+        if (p.c.part_o) {
+          const long at = (static_cast<long>(p.c.slot0 + t.split) * p.c.B * p.c.Sq + token) * p.c.H + head;
+          if (row_ok) p.c.part_lse[at] = lse2;
+          if (t.nb > 0) {
+            for (int c = 0; c < DK / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld_32x16(tmem_o + c * 16, o);
               tmem_ld_wait();
-            } else {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = 0;
-            }
-            if (lane == 0) tma_store_wait_read1();
-            __syncwarp();
-            uint8_t* buf = stage + (nout++ & 1) * 2048;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              uint4 v;
-              v.x = ctx_pack2<FP16>(__uint_as_float(o[x * 8 + 0]) * inv, __uint_as_float(o[x * 8 + 1]) * inv);
-              v.y = ctx_pack2<FP16>(__uint_as_float(o[x * 8 + 2]) * inv, __uint_as_float(o[x * 8 + 3]) * inv);
-              v.z = ctx_pack2<FP16>(__uint_as_float(o[x * 8 + 4]) * inv, __uint_as_float(o[x * 8 + 5]) * inv);
-              v.w = ctx_pack2<FP16>(__uint_as_float(o[x * 8 + 6]) * inv, __uint_as_float(o[x * 8 + 7]) * inv);
-              *reinterpret_cast<uint4*>(buf + lane * 64 + ((x ^ ((lane >> 1) & 3)) << 4)) = v;
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            const int first_tok = tile_tok + (warp & 3) * 32 / p.pack;
-            if (lane == 0 && first_tok < p.c.Sq) {
-              tma_store_4d(&tmO, buf, c * 32, t.hg * p.pack, first_tok, t.b);
-              tma_store_commit();
+              for (int e = 0; e < 16; e += 4)
+                if (row_ok && c * 16 + e < p.c.D)
+                  *reinterpret_cast<float4*>(p.c.part_o + at * p.c.D + c * 16 + e) =
+                      make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv,
+                                  __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
             }
           }
+        } else {
+          if (p.c.lse && row_ok)
+            p.c.lse[(static_cast<long>(t.b) * p.c.H + head) * p.c.Sq + tok] = lse2 * 0.6931471805599453f;
+          if (lane == 0) tma_store_wait_read0();  // the boxes of the previous tile have left
+          __syncwarp();
+          const int first_tok = tile_tok + wq * 32 / p.pack;
+#pragma unroll
+          for (int x = 0; x < NBOX; ++x) {
+            if (x * 64 < p.c.D) {
+              uint8_t* buf = stage + x * 4096 + lane * 128;
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                uint32_t o[16];
+                if (t.nb > 0) {
+                  tmem_ld_32x16(tmem_o + x * 64 + c * 16, o);
+                  tmem_ld_wait();
+                } else {
+#pragma unroll
+                  for (int e = 0; e < 16; ++e) o[e] = 0;
+                }
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                  uint4 v;
+                  v.x = ctx_pack2<FP16>(__uint_as_float(o[y * 8 + 0]) * inv, __uint_as_float(o[y * 8 + 1]) * inv);
+                  v.y = ctx_pack2<FP16>(__uint_as_float(o[y * 8 + 2]) * inv, __uint_as_float(o[y * 8 + 3]) * inv);
+                  v.z = ctx_pack2<FP16>(__uint_as_float(o[y * 8 + 4]) * inv, __uint_as_float(o[y * 8 + 5]) * inv);
+                  v.w = ctx_pack2<FP16>(__uint_as_float(o[y * 8 + 6]) * inv, __uint_as_float(o[y * 8 + 7]) * inv);
+                  *reinterpret_cast<uint4*>(buf + (((c * 2 + y) ^ (lane & 7)) << 4)) = v;  // 128B swizzle
+                }
+              }
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0 && first_tok < p.c.Sq) {
+                tma_store_4d(&tmO, stage + x * 4096, x * 64, t.hg * p.pack, first_tok, t.b);
+                tma_store_commit();
+              }
+            }
+          }
+        }
+        if (t.nb > 0) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&o_empty[st]);
         }
       }
     }
     if (lane == 0) tma_store_wait_all();
     __syncwarp();
+  } else if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 0) {
+      // ------------------------------ TMA loader ------------------------------
+      const bool leader = lane == 0;
+      if (leader) {
+        tma_prefetch_desc(&tmQ);
+        tma_prefetch_desc(&tmK);
+        tma_prefetch_desc(&tmV);
+      }
+      int g = 0;             // key blocks so far
+      uint32_t q_phase = 3;  // bit per query tile; a barrier that was never used lets its first waiter through
+      int v_row = 0, v_b = 0, v_hk = 0;
+      bool v_pre = false, ok = true;
+      auto load = [&](const CUtensorMap* tm, int off, uint64_t* bar, int hk, int row, int b) {
+        for (int x = 0; x < NBOX; ++x) tma_load_4d(smem + off + x * CT_BOX, tm, bar, x * 64, hk, row, b);
+      };
+      while (ok && items.next(t, ctx, 40)) {
+        const int hk = t.hg * p.pack / (p.c.H / p.c.Hkv);
+        for (int n = 0; n < t.nb; ++n, ++g) {
+          const int j = t.j0 + n;
+          const bool pre = j < p.n_prefix;
+          const int row = pre ? j * 128 : t.first + (j - p.n_prefix) * 128;
+          const int bb = pre ? 0 : t.b * p.bmul;
+          const CUtensorMap* tk = pre ? &tmKp : &tmK;
+          if (g == 0) {
+            if (leader) {
+              mbar_expect_tx(k_first, LOAD_BYTES);
+              load(tk, CT_KV_OFF, k_first, hk, row, bb);
+            }
+          } else {  // stage g - 1: V of the block before, K of this one
+            const int slot = (g - 1) & 1;
+            if (!(ok = mbar_wait_warp(&kv_empty[slot], (((g - 1) >> 1) & 1) ^ 1, ctx, 41))) break;
+            if (leader) {
+              mbar_expect_tx(&kv_full[slot], 2 * LOAD_BYTES);
+              load(v_pre ? &tmVp : &tmV, CT_KV_OFF + (2 + slot) * CT_TILE, &kv_full[slot], v_hk, v_row, v_b);
+              load(tk, CT_KV_OFF + (g & 1) * CT_TILE, &kv_full[slot], hk, row, bb);
+            }
+          }
+          v_pre = pre, v_hk = hk, v_row = row, v_b = bb;
+          if (n == 0) {
+            for (int st = 0; st < (t.two(p) ? 2 : 1); ++st) {
+              if (!(ok = mbar_wait_warp(&q_empty[st], (q_phase >> st) & 1, ctx, 42))) break;
+              q_phase ^= 1u << st;
+              if (leader) {
+                mbar_expect_tx(&q_full[st], LOAD_BYTES);
+                load(&tmQ, CT_Q_OFF + st * CT_TILE, &q_full[st], t.hg * p.pack, (t.qp * 2 + st) * p.tok, t.b);
+              }
+            }
+            if (!ok) break;
+          }
+          __syncwarp();
+        }
+      }
+      if (ok && g > 0) {  // the last block's V has no K beside it
+        const int slot = (g - 1) & 1;
+        if (mbar_wait_warp(&kv_empty[slot], (((g - 1) >> 1) & 1) ^ 1, ctx, 43) && leader) {
+          mbar_expect_tx(&kv_full[slot], LOAD_BYTES);
+          load(v_pre ? &tmVp : &tmV, CT_KV_OFF + (2 + slot) * CT_TILE, &kv_full[slot], v_hk, v_row, v_b);
+        }
+        __syncwarp();
+      }
+    } else if (warp == 1) {
+      // ------------------------------ MMA issuer ------------------------------
+      constexpr uint32_t FMT = FP16 ? 0 : 1;
+      constexpr uint32_t idesc_pv = make_idesc(128, DK, FMT, FMT, 0, 1);  // B (= V) is MN-major
+      // A descriptor holds its address in units of 16 bytes in the low bits, so tiles and k-steps are reached by addition.
+      const uint64_t q_desc = make_desc_k_sw128(smem_u32(smem + CT_Q_OFF));
+      const uint64_t k_desc = make_desc_k_sw128(smem_u32(smem + CT_KV_OFF));
+      const uint64_t v_desc = make_desc_mn_sw128(smem_u32(smem + CT_KV_OFF + 2 * CT_TILE), CT_BOX);
+      CtxItem nt;
+      int g = 0;
+      uint32_t q_phase = 0, p_phase = 0, o_phase = 3;  // bit per query tile
+      bool ok = true;
+      // the next item with keys
+      auto next_item = [&](CtxItem& it) {
+        while (items.next(it, ctx, 44))
+          if (it.nb > 0) return true;
+        return false;
+      };
+      // one lane: Q.K^T of `cols` columns of ring block gg into S of query tile st; `last`: the item's last block
+      auto issue_qk = [&](int st, int gg, int cols, bool last) {
+        const uint32_t idesc = make_idesc(128, 0, FMT, FMT, 0, 0) | (static_cast<uint32_t>(cols >> 3) << 17);
+        const uint64_t qd = q_desc + st * (CT_TILE >> 4), kd = k_desc + (gg & 1) * (CT_TILE >> 4);
+        const uint32_t d = tmem_base + st * 128;
+#pragma unroll
+        for (int kk = 0; kk < DK / 16; ++kk) {
+          const uint32_t off = ((kk >> 2) * CT_BOX + (kk & 3) * 32) >> 4;
+          umma_f16_ss(d, qd + off, kd + off, idesc, kk ? 1u : 0u);
+        }
+        umma_commit(&s_full[st]);
+        if (last) umma_commit(&q_empty[st]);
+      };
+      auto cols_of = [&](const CtxItem& it, int n) { return (ctx_block_keys(p, it.j0 + n, it.len) + 31) & ~31; };
+      // First scores of an item; its K is already there.
+      auto prime = [&](int st, const CtxItem& it, int gg) {
+        if (!mbar_wait_warp(&q_full[st], (q_phase >> st) & 1, ctx, 45)) return false;
+        q_phase ^= 1u << st;
+        tc_fence_after();
+        if (elect_one()) issue_qk(st, gg, cols_of(it, 0), it.nb == 1);
+        __syncwarp();
+        return true;
+      };
+      bool have = next_item(t);
+      if (have)
+        ok = mbar_wait_warp(k_first, 0, ctx, 46) && prime(0, t, 0) && (!t.two(p) || prime(1, t, 0));
+      while (have && ok) {
+        const int gn = g + t.nb, tiles = t.two(p) ? 2 : 1;
+        const bool have_next = next_item(nt);
+        const int next_tiles = !have_next ? 0 : nt.two(p) ? 2 : 1;
+        int cols = cols_of(t, 0);
+        for (; g < gn && ok; ++g) {
+          const bool first = g + t.nb == gn, more = g + 1 < gn;
+          const int steps = cols >> 4;
+          if (more) cols = cols_of(t, g + 1 - (gn - t.nb));
+          if (!(ok = mbar_wait_warp(&kv_ready[g & 1], (g >> 1) & 1, ctx, 47))) break;
+          const uint64_t vd = v_desc + (g & 1) * (CT_TILE >> 4);
+          for (int st = 0; st < tiles; ++st) {
+            if (first) {  // the accumulator of the tile's previous item has been read
+              if (!(ok = mbar_wait_warp(&o_empty[st], (o_phase >> st) & 1, ctx, 48))) break;
+              o_phase ^= 1u << st;
+            }
+            if (!(ok = mbar_wait_warp(&p_ready[st], (p_phase >> st) & 1, ctx, 49))) break;
+            p_phase ^= 1u << st;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint32_t o_tmem = tmem_base + 256 + st * 128, p_tmem = tmem_base + st * 128;
+              if (steps == 8) {
+#pragma unroll
+                for (int kk = 0; kk < 8; ++kk)
+                  umma_f16_ts(o_tmem, p_tmem + kk * 8, vd + kk * (2048 >> 4), idesc_pv, kk ? 1u : first ? 0u : 1u);
+              } else {
+                for (int kk = 0; kk < steps; ++kk)
+                  umma_f16_ts(o_tmem, p_tmem + kk * 8, vd + kk * (2048 >> 4), idesc_pv, kk ? 1u : first ? 0u : 1u);
+              }
+              if (more)
+                issue_qk(st, g + 1, cols, g + 2 == gn);
+              else
+                umma_commit(&o_final[st]);
+            }
+            __syncwarp();
+            if (!more && st < next_tiles && !(ok = prime(st, nt, gn))) break;
+          }
+          if (ok && !more && tiles < next_tiles) ok = prime(1, nt, gn);
+          if (ok && elect_one()) umma_commit(&kv_empty[g & 1]);
+          __syncwarp();
+        }
+        have = have_next;
+        t = nt;
+      }
+    } else if (warp == 2) {
+      // ------------------------------ tail / mask warp ------------------------------
+      int g = 0;
+      bool ok = true;
+      while (ok && items.next(t, ctx, 52)) {
+        for (int n = 0; n < t.nb; ++n, ++g) {
+          const int slot = g & 1, j = t.j0 + n;
+          const int keys = ctx_block_keys(p, j, t.len);
+          uint32_t w[4];
+          if (MASK) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int key = x * 32 + lane;
+              bool vis = key < keys;
+              if (vis) vis = __ldg(p.c.key_mask + static_cast<long>(t.b) * p.c.mask_bs + j * 128L + key) != 0;
+              w[x] = __ballot_sync(0xffffffffu, vis);
+            }
+          }
+          if (!(ok = mbar_wait_warp(&kv_full[slot], (g >> 1) & 1, ctx, 53))) break;
+          bool wrote = false;
+          if (MASK || keys < 128) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int left = keys - x * 32;
+              const uint32_t vis = MASK ? w[x] : left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
+              if (left > 0 && vis != 0xffffffffu) {  // steps without a key are not read
+                wrote = true;
+                if (!((vis >> lane) & 1)) {
+                  uint4* row = reinterpret_cast<uint4*>(smem + CT_KV_OFF + (2 + slot) * CT_TILE + (x * 32 + lane) * 128);
+#pragma unroll
+                  for (int y = 0; y < NBOX; ++y)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) row[y * (CT_BOX / 16) + e] = make_uint4(0, 0, 0, 0);
+                }
+              }
+              if (MASK && lane == x) words[slot * 4 + x] = vis;
+            }
+          }
+          if (wrote) fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&kv_ready[slot]);
+        }
+      }
+    } else if (warp == 3) {
+      // ------------------------------ item decoder ------------------------------
+      int4* ring = reinterpret_cast<int4*>(smem + CT_ITEM_OFF);
+      if (lane == 0) {
+        int n = 0;
+        for (int i = blockIdx.x;; i += gridDim.x, ++n) {
+          const bool end = i >= p.n_items;
+          if (!end)
+            t = ctx_item(p, i);
+          else
+            t.b = -1, t.hg = t.qp = t.split = t.first = t.len = t.j0 = t.nb = 0;
+          const int slot = n % CT_ITEMS;
+          if (!mbar_wait(&i_empty[slot], ((n / CT_ITEMS) & 1) ^ 1, ctx, 54)) break;
+          ring[slot * 2] = make_int4(t.b, t.hg, t.qp, t.split);
+          ring[slot * 2 + 1] = make_int4(t.first, t.len, t.j0, t.nb);
+          mbar_arrive(&i_full[slot]);
+          if (end) break;
+        }
+      }
+      __syncwarp();
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+    // ------------------------------ softmax groups ------------------------------
+    const int st = (warp >> 2) - 1;
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tmem_s = tmem_base + lane_addr + st * 128;
+    const uint32_t tmem_o = tmem_base + lane_addr + 256 + st * 128;
+    int ns = 0, no = 0, g = 0;  // score tiles, items with keys and key blocks seen so far
+    bool ok = true;
+    while (ok && items.next(t, ctx, 58)) {
+      if (t.nb == 0) continue;
+      if (st && !t.two(p)) {
+        g += t.nb;
+        continue;
+      }
+      float m_used = -INFINITY, l = 0.f;
+      for (int n = 0; n < t.nb; ++n, ++g) {
+        const int keys = ctx_block_keys(p, t.j0 + n, t.len);
+        if (!(ok = mbar_wait_warp(&s_full[st], ns & 1, ctx, 59))) break;
+        ++ns;
+        tc_fence_after();
+        bool part = keys < 128;
+        volatile const uint32_t* w = words + (g & 1) * 4;
+        if (MASK) {
+          // behind s_full: the scores of block g exist only once kv_ready of block g - 1 has completed, so the parity of
+          // block g cannot be mistaken for that of block g - 4 by a group that skipped items
+          if (!(ok = mbar_wait_warp(&kv_ready[g & 1], (g >> 1) & 1, ctx, 60))) break;
+          part = part || (w[0] & w[1] & w[2] & w[3]) != 0xffffffffu;
+        }
+        if (part)
+          ctx_softmax_part<FP16, DK, MASK>(tmem_s, tmem_o, p.c.scale_log2, keys, w, n == 0, m_used, l);
+        else
+          ctx_softmax_full<FP16, DK>(tmem_s, tmem_o, p.c.scale_log2, n == 0, m_used, l);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&p_ready[st]);
+      }
+      if (!ok) break;
+      if (!(ok = mbar_wait_warp(&o_empty[st], (no & 1) ^ 1, ctx, 61))) break;  // the previous item's have been read
+      ++no;
+      ml[st * 128 + row] = make_float2(m_used, l);
+      mbar_arrive(&l_full[st]);
+    }
   }
 
   if (*abort_flag) __nanosleep(200000);
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) tmem_dealloc(tmem_base, 512);
+  if (warp == 1) tmem_dealloc(tmem_base, 512);
 }
 
 static int ctx_pack(int G) { return (G & (G - 1)) == 0 && G <= 32 ? G : 1; }
@@ -516,7 +666,7 @@ static int launch_ctx_tc_impl(const CUtensorMap (&tm)[6], const CtxTcParams& p, 
   auto kern = &ctx_tc_kernel<FP16, DK, MASK>;
   if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), CT_SMEM_BYTES, attr_set)) return rc;
   const int grid = p.n_items < sm_count() ? p.n_items : sm_count();
-  kern<<<grid, 384, CT_SMEM_BYTES, st>>>(tm[0], tm[1], tm[2], tm[3], tm[4], tm[5], p);
+  kern<<<grid, 512, CT_SMEM_BYTES, st>>>(tm[0], tm[1], tm[2], tm[3], tm[4], tm[5], p);
   return cudaGetLastError() == cudaSuccess ? TFB_OK : TFB_ERR_LAUNCH;
 }
 
@@ -552,7 +702,7 @@ int launch_ctx_tc(const CtxParams& c, const void* kp, long kp_ss, long kp_hs, co
   if (c.part_o) {
     tm[5] = tm[0];
   } else if ((e = ctx_tmap(&tm[5], c.out, fp16, c.D, c.H, c.D, c.Sq, static_cast<long>(c.H) * c.D, c.B,
-                           static_cast<long>(c.Sq) * c.H * c.D, 32, p.pack, 32 / p.pack, TM_SW_64))) {
+                           static_cast<long>(c.Sq) * c.H * c.D, 64, p.pack, 32 / p.pack, TM_SW_128))) {
     return e;
   }
   const bool mask = c.key_mask != nullptr;
