@@ -36,9 +36,9 @@ constexpr int CT_ML_OFF = CT_OUT_OFF + 4 * 8192;     // [2 tiles][128 rows] of (
 constexpr int CT_ITEMS = 4;                          // ring of decoded items
 constexpr int CT_ITEM_OFF = CT_ML_OFF + 2 * 128 * 8;
 constexpr int CT_BAR_OFF = CT_ITEM_OFF + CT_ITEMS * 32;
-constexpr int CT_N_BARS = 21 + 2 * CT_ITEMS;
+constexpr int CT_N_BARS = 20 + 2 * CT_ITEMS;
 constexpr int CT_ALIGN_SLACK = 512;  // dynamic shared memory starts on 1 KB here; the kernel checks that the tiles fit
-constexpr int CT_SMEM_BYTES = CT_BAR_OFF + (CT_N_BARS + 1) * 8 + 64 + CT_ALIGN_SLACK;
+constexpr int CT_SMEM_BYTES = CT_BAR_OFF + CT_N_BARS * 8 + 64 + CT_ALIGN_SLACK;
 static_assert(CT_SMEM_BYTES <= 227 * 1024, "shared memory of one CTA");
 constexpr int CT_ITEM_READERS = 3 + 8 + 4;  // loader, issuer and tail warp, softmax warps, output warps
 constexpr float CT_RESCALE_THRESHOLD = 8.0f;
@@ -229,18 +229,17 @@ __global__ void __launch_bounds__(512, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + CT_BAR_OFF);
   uint64_t* q_full = bars + 0;     // [2] per query tile
   uint64_t* q_empty = bars + 2;    // [2]
-  uint64_t* kv_full = bars + 4;    // [2] stage g & 1: V of key block g and K of block g + 1
-  uint64_t* kv_ready = bars + 6;   // [2] ... with the hidden V rows cleared and the mask words of block g written
+  uint64_t* kv_full = bars + 4;    // [2] stage s, in slot s & 1: K of key block s and V of block s - 1
+  uint64_t* kv_ready = bars + 6;   // [2] ... with the hidden V rows cleared and the mask words of block s - 1 written
   uint64_t* kv_empty = bars + 8;   // [2]
   uint64_t* s_full = bars + 10;    // [2] per query tile
   uint64_t* p_ready = bars + 12;   // [2]
   uint64_t* o_final = bars + 14;   // [2] the tile's last P.V is done
   uint64_t* l_full = bars + 16;    // [2] the tile's maxima and sums are in shared memory
   uint64_t* o_empty = bars + 18;   // [2] accumulator, maxima and sums have been read
-  uint64_t* k_first = bars + 20;   // K of block 0
-  uint64_t* i_full = bars + 21;    // [CT_ITEMS]
+  uint64_t* i_full = bars + 20;    // [CT_ITEMS]
   uint64_t* i_empty = i_full + CT_ITEMS;
-  uint32_t* words = reinterpret_cast<uint32_t*>(bars + ((CT_N_BARS + 1) & ~1));  // [2 slots][4]
+  uint32_t* words = reinterpret_cast<uint32_t*>(bars + CT_N_BARS);  // [2 slots][4]
   uint32_t* tmem_slot = words + 8;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float2* ml = reinterpret_cast<float2*>(smem + CT_ML_OFF);
@@ -262,7 +261,6 @@ __global__ void __launch_bounds__(512, 1)
       mbar_init(&l_full[s], 128);
       mbar_init(&o_empty[s], 4);
     }
-    mbar_init(k_first, 1);
     for (int s = 0; s < CT_ITEMS; ++s) {
       mbar_init(&i_full[s], 1);
       mbar_init(&i_empty[s], CT_ITEM_READERS);
@@ -400,20 +398,12 @@ __global__ void __launch_bounds__(512, 1)
           const bool pre = j < p.n_prefix;
           const int row = pre ? j * 128 : t.first + (j - p.n_prefix) * 128;
           const int bb = pre ? 0 : t.b * p.bmul;
-          const CUtensorMap* tk = pre ? &tmKp : &tmK;
-          if (g == 0) {
-            if (leader) {
-              mbar_expect_tx(k_first, LOAD_BYTES);
-              load(tk, CT_KV_OFF, k_first, hk, row, bb);
-            }
-          } else {  // stage g - 1: V of the block before, K of this one
-            const int slot = (g - 1) & 1;
-            if (!(ok = mbar_wait_warp(&kv_empty[slot], (((g - 1) >> 1) & 1) ^ 1, ctx, 41))) break;
-            if (leader) {
-              mbar_expect_tx(&kv_full[slot], 2 * LOAD_BYTES);
-              load(v_pre ? &tmVp : &tmV, CT_KV_OFF + (2 + slot) * CT_TILE, &kv_full[slot], v_hk, v_row, v_b);
-              load(tk, CT_KV_OFF + (g & 1) * CT_TILE, &kv_full[slot], hk, row, bb);
-            }
+          const int slot = g & 1;  // stage g
+          if (!(ok = mbar_wait_warp(&kv_empty[slot], ((g >> 1) & 1) ^ 1, ctx, 41))) break;
+          if (leader) {
+            mbar_expect_tx(&kv_full[slot], (g > 0 ? 2 : 1) * LOAD_BYTES);
+            if (g > 0) load(v_pre ? &tmVp : &tmV, CT_KV_OFF + (2 + slot) * CT_TILE, &kv_full[slot], v_hk, v_row, v_b);
+            load(pre ? &tmKp : &tmK, CT_KV_OFF + slot * CT_TILE, &kv_full[slot], hk, row, bb);
           }
           v_pre = pre, v_hk = hk, v_row = row, v_b = bb;
           if (n == 0) {
@@ -431,8 +421,8 @@ __global__ void __launch_bounds__(512, 1)
         }
       }
       if (ok && g > 0) {  // the last block's V has no K beside it
-        const int slot = (g - 1) & 1;
-        if (mbar_wait_warp(&kv_empty[slot], (((g - 1) >> 1) & 1) ^ 1, ctx, 43) && leader) {
+        const int slot = g & 1;
+        if (mbar_wait_warp(&kv_empty[slot], ((g >> 1) & 1) ^ 1, ctx, 43) && leader) {
           mbar_expect_tx(&kv_full[slot], LOAD_BYTES);
           load(v_pre ? &tmVp : &tmV, CT_KV_OFF + (2 + slot) * CT_TILE, &kv_full[slot], v_hk, v_row, v_b);
         }
@@ -480,8 +470,11 @@ __global__ void __launch_bounds__(512, 1)
         return true;
       };
       bool have = next_item(t);
-      if (have)
-        ok = mbar_wait_warp(k_first, 0, ctx, 46) && prime(0, t, 0) && (!t.two(p) || prime(1, t, 0));
+      if (have) {
+        ok = mbar_wait_warp(&kv_ready[0], 0, ctx, 46) && prime(0, t, 0) && (!t.two(p) || prime(1, t, 0));
+        if (ok && elect_one()) umma_commit(&kv_empty[0]);
+        __syncwarp();
+      }
       while (have && ok) {
         const int gn = g + t.nb, tiles = t.two(p) ? 2 : 1;
         const bool have_next = next_item(nt);
@@ -491,8 +484,9 @@ __global__ void __launch_bounds__(512, 1)
           const bool first = g + t.nb == gn, more = g + 1 < gn;
           const int steps = cols >> 4;
           if (more) cols = cols_of(t, g + 1 - (gn - t.nb));
-          if (!(ok = mbar_wait_warp(&kv_ready[g & 1], (g >> 1) & 1, ctx, 47))) break;
-          const uint64_t vd = v_desc + (g & 1) * (CT_TILE >> 4);
+          const int slot = (g + 1) & 1;  // stage g + 1: V of this block and K of the next
+          if (!(ok = mbar_wait_warp(&kv_ready[slot], ((g + 1) >> 1) & 1, ctx, 47))) break;
+          const uint64_t vd = v_desc + slot * (CT_TILE >> 4);
           for (int st = 0; st < tiles; ++st) {
             if (first) {  // the accumulator of the tile's previous item has been read
               if (!(ok = mbar_wait_warp(&o_empty[st], (o_phase >> st) & 1, ctx, 48))) break;
@@ -520,7 +514,7 @@ __global__ void __launch_bounds__(512, 1)
             if (!more && st < next_tiles && !(ok = prime(st, nt, gn))) break;
           }
           if (ok && !more && tiles < next_tiles) ok = prime(1, nt, gn);
-          if (ok && elect_one()) umma_commit(&kv_empty[g & 1]);
+          if (ok && elect_one()) umma_commit(&kv_empty[slot]);
           __syncwarp();
         }
         have = have_next;
@@ -531,7 +525,12 @@ __global__ void __launch_bounds__(512, 1)
       int g = 0;
       bool ok = true;
       while (ok && items.next(t, ctx, 52)) {
-        for (int n = 0; n < t.nb; ++n, ++g) {
+        for (int n = 0; n < t.nb; ++n) {
+          if (g == 0) {  // stage 0 has no V
+            if (!(ok = mbar_wait_warp(&kv_full[0], 0, ctx, 62))) break;
+            if (lane == 0) mbar_arrive(&kv_ready[0]);
+          }
+          ++g;  // the stage with this block's V
           const int slot = g & 1, j = t.j0 + n;
           const int keys = ctx_block_keys(p, j, t.len);
           uint32_t w[4];
@@ -613,11 +612,11 @@ __global__ void __launch_bounds__(512, 1)
         ++ns;
         tc_fence_after();
         bool part = keys < 128;
-        volatile const uint32_t* w = words + (g & 1) * 4;
+        volatile const uint32_t* w = words + ((g + 1) & 1) * 4;
         if (MASK) {
-          // behind s_full: the scores of block g exist only once kv_ready of block g - 1 has completed, so the parity of
-          // block g cannot be mistaken for that of block g - 4 by a group that skipped items
-          if (!(ok = mbar_wait_warp(&kv_ready[g & 1], (g >> 1) & 1, ctx, 60))) break;
+          // Behind s_full: the scores of block g exist only once stage g was ready, so stage g - 1 was too, and the parity
+          // of stage g + 1 cannot be mistaken for that of stage g - 3 by a group that skipped items.
+          if (!(ok = mbar_wait_warp(&kv_ready[(g + 1) & 1], ((g + 1) >> 1) & 1, ctx, 60))) break;
           part = part || (w[0] & w[1] & w[2] & w[3]) != 0xffffffffu;
         }
         if (part)
