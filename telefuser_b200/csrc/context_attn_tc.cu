@@ -525,23 +525,31 @@ __global__ void __launch_bounds__(512, 1)
       int g = 0;
       bool ok = true;
       while (ok && items.next(t, ctx, 52)) {
+        // mask bytes of the item's block n, this lane's four keys; loaded one block ahead of their use
+        auto load_mask = [&](int n, uint8_t (&m)[4]) {
+          const int j = t.j0 + n, keys = ctx_block_keys(p, j, t.len);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            m[x] = 0;
+            if (x * 32 + lane < keys)
+              m[x] = __ldg(p.c.key_mask + static_cast<long>(t.b) * p.c.mask_bs + j * 128L + x * 32 + lane);
+          }
+        };
+        uint8_t m[4];
+        if (MASK && t.nb > 0) load_mask(0, m);
         for (int n = 0; n < t.nb; ++n) {
           if (g == 0) {  // stage 0 has no V
             if (!(ok = mbar_wait_warp(&kv_full[0], 0, ctx, 62))) break;
             if (lane == 0) mbar_arrive(&kv_ready[0]);
           }
           ++g;  // the stage with this block's V
-          const int slot = g & 1, j = t.j0 + n;
-          const int keys = ctx_block_keys(p, j, t.len);
+          const int slot = g & 1;
+          const int keys = ctx_block_keys(p, t.j0 + n, t.len);
           uint32_t w[4];
           if (MASK) {
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const int key = x * 32 + lane;
-              bool vis = key < keys;
-              if (vis) vis = __ldg(p.c.key_mask + static_cast<long>(t.b) * p.c.mask_bs + j * 128L + key) != 0;
-              w[x] = __ballot_sync(0xffffffffu, vis);
-            }
+            for (int x = 0; x < 4; ++x) w[x] = __ballot_sync(0xffffffffu, m[x] != 0);
+            if (n + 1 < t.nb) load_mask(n + 1, m);
           }
           if (!(ok = mbar_wait_warp(&kv_full[slot], (g >> 1) & 1, ctx, 53))) break;
           bool wrote = false;

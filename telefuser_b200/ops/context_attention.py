@@ -15,24 +15,18 @@ Role parity: telefuser/ops/attention/attention_impl.py:112-315 (variable-length 
 
 from __future__ import annotations
 
-import ctypes
+import functools
 import math
+import struct
 
 import torch
 
 from . import native
 from .functional import _native
 
-_NAMES = ("q", "k", "v", "kp", "vp", "out", "lse", "kv_lens", "cu_kv", "key_mask", "work")
-_LONGS = ("q_bs", "q_ss", "q_hs", "k_bs", "k_ss", "k_hs", "v_bs", "v_ss", "v_hs", "kp_ss", "kp_hs", "vp_ss", "vp_hs", "mask_bs")
-_INTS = ("B", "Sq", "H", "Hkv", "D", "Skv", "P", "fp16")
-
-
-class _Args(ctypes.Structure):
-    """tfb_context_attn_args of csrc/tfb_api.h."""
-
-    _fields_ = ([(n, ctypes.c_void_p) for n in _NAMES] + [(n, ctypes.c_long) for n in _LONGS]
-                + [(n, ctypes.c_int) for n in _INTS] + [("scale", ctypes.c_float), ("reserved", ctypes.c_int)])  # fmt: skip
+# tfb_context_attn_args of csrc/tfb_api.h: 11 pointers, 14 strides, 8 sizes, the scale, one reserved word. Packed in one
+# step: a ctypes structure filled field by field costs a short call several microseconds.
+_ARGS = struct.Struct("@11P14l8ifi")
 
 
 def context_attention_reference(q, k, v, visible=None, scale=None, return_lse=False, q_block: int | None = None):
@@ -66,10 +60,11 @@ def _q_block(q, keys: int) -> int | None:
 
 
 def _check(q, k, v, what: str) -> None:
-    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
-        raise ValueError(f"{what}: q [B, Sq, H, D] and k / v of one shape [B, Skv, Hkv, D], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    if k.shape[3] != q.shape[3] or k.shape[2] < 1 or q.shape[2] % k.shape[2]:
-        raise ValueError(f"{what}: heads {q.shape[2]} x {q.shape[3]} do not fit key heads {k.shape[2]} x {k.shape[3]}")
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or ks != v.shape:
+        raise ValueError(f"{what}: q [B, Sq, H, D] and k / v of one shape [B, Skv, Hkv, D], got {tuple(qs)}, {tuple(ks)}, {tuple(v.shape)}")
+    if ks[3] != qs[3] or ks[2] < 1 or qs[2] % ks[2]:
+        raise ValueError(f"{what}: heads {qs[2]} x {qs[3]} do not fit key heads {ks[2]} x {ks[3]}")
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError(f"{what}: q, k and v have one type, got {q.dtype}, {k.dtype}, {v.dtype}")
     native.same_device(q, k, v)
@@ -96,55 +91,63 @@ def _lengths(lens, n: int, most: int, device, what: str):
     return lens.contiguous() if lens.dtype == torch.int32 else lens.clamp(-1, 2**31 - 1).to(torch.int32)
 
 
-def _strided(t):
-    """t with unit channel stride, 16-byte rows and no broadcast dimension, copied only if it is not so already."""
-    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0
-    for n, s in zip(t.shape[:-1], t.stride()[:-1]):
-        ok = ok and (n <= 1 or (s > 0 and s % 8 == 0))
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
-
-
-def _stride(t, dim: int) -> int:
-    return t.stride(dim) if t.shape[dim] > 1 else 0
+def _operand(t):
+    """-> (tensor, address, batch, token and head strides), with unit channel stride, 16-byte rows and no broadcast dimension:
+    copied only if it is not so already. A dimension of one entry gets stride 0."""
+    at = t.data_ptr()
+    B, S, H, D = t.shape
+    if t.is_contiguous() and at % 16 == 0 and D % 8 == 0:
+        return t, at, S * H * D, H * D, D
+    strides = [s if n > 1 else 0 for n, s in zip(t.shape, t.stride())]
+    if at % 16 or (D > 1 and strides[3] != 1) or any(n > 1 and (s <= 0 or s % 8) for n, s in zip(t.shape[:3], strides)):
+        return _operand(t.clone(memory_format=torch.contiguous_format))
+    return t, at, strides[0], strides[1], strides[2]
 
 
 def _runs_native(q) -> bool:
     return _native(q) and q.dtype in (torch.bfloat16, torch.float16) and q.shape[3] % 8 == 0 and 8 <= q.shape[3] <= 128
 
 
+@functools.lru_cache(maxsize=4096)
+def _work_bytes(device: int, packed: bool, masked: bool, sizes: tuple) -> int:
+    """Scratch of a call of these sizes (the key splits depend on nothing else)."""
+    some = 16  # an address that is not looked at
+    args = _ARGS.pack(some, some, some, some, some, some, 0, 0, some if packed else 0, some if masked else 0, 0, *(0,) * 14,
+                      *sizes, 1.0, 0)  # fmt: skip
+    need = native.load().tfb_context_attn_work(args)
+    if need < 0:
+        native.check(-need, "tfb_context_attn_work")
+    return need
+
+
 def _launch(q, k, v, kp, vp, kv_lens, cu_kv, key_mask, scale, return_lse):
-    if q.device.index != torch.cuda.current_device():
-        with torch.cuda.device(q.device):
+    dev = q.device.index
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
             return _launch(q, k, v, kp, vp, kv_lens, cu_kv, key_mask, scale, return_lse)
     B, Sq, H, D = q.shape
-    a = _Args()
-    if B > 1 and Sq > 1 and kp is not None and q.stride(0) != Sq * q.stride(1):
+    P = 0 if kp is None else kp.shape[1]
+    if P and B > 1 and Sq > 1 and q.stride(0) != Sq * q.stride(1):
         q = q.contiguous()  # the shared prefix sees the tokens of all samples as one row after the other
-    q, k, v = _strided(q), _strided(k), _strided(v)
-    a.q, a.q_bs, a.q_ss, a.q_hs = q.data_ptr(), _stride(q, 0), _stride(q, 1), _stride(q, 2)
-    a.k, a.k_bs, a.k_ss, a.k_hs = k.data_ptr(), _stride(k, 0), _stride(k, 1), _stride(k, 2)
-    a.v, a.v_bs, a.v_ss, a.v_hs = v.data_ptr(), _stride(v, 0), _stride(v, 1), _stride(v, 2)
-    a.B, a.Sq, a.H, a.Hkv, a.D, a.Skv = B, Sq, H, k.shape[2], D, k.shape[1]
-    a.fp16, a.scale = int(q.dtype == torch.float16), scale
-    if kp is not None and kp.shape[1]:
-        kp, vp = _strided(kp), _strided(vp)
-        a.kp, a.kp_ss, a.kp_hs, a.vp, a.vp_ss, a.vp_hs = (kp.data_ptr(), _stride(kp, 1), _stride(kp, 2), vp.data_ptr(),
-                                                          _stride(vp, 1), _stride(vp, 2))  # fmt: skip
-        a.P = kp.shape[1]
-    a.kv_lens, a.cu_kv, a.key_mask = native.ptr(kv_lens), native.ptr(cu_kv), native.ptr(key_mask)
-    if key_mask is not None:
-        a.mask_bs = key_mask.stride(0)
-    out = torch.empty(B, Sq, H, D, device=q.device, dtype=q.dtype)
-    lse = torch.empty(B, H, Sq, device=q.device, dtype=torch.float32) if return_lse else None
-    if out.numel():
-        a.out, a.lse = out.data_ptr(), native.ptr(lse)
-        lib = native.load()
-        need = lib.tfb_context_attn_work(ctypes.byref(a))
-        if need < 0:
-            native.check(-need, "tfb_context_attn_work")
+    out = torch.empty((B, Sq, H, D), device=q.device, dtype=q.dtype)
+    lse = torch.empty((B, H, Sq), device=q.device, dtype=torch.float32) if return_lse else None
+    if B and Sq and H:
+        q, qp, q_bs, q_ss, q_hs = _operand(q)
+        k, kk, k_bs, k_ss, k_hs = _operand(k)
+        v, vv, v_bs, v_ss, v_hs = _operand(v)
+        pre = (0, 0, 0, 0, 0, 0)
+        if P:
+            kp, a, _, a_ss, a_hs = _operand(kp)
+            vp, b, _, b_ss, b_hs = _operand(vp)
+            pre = (a, b, a_ss, a_hs, b_ss, b_hs)
+        sizes = (B, Sq, H, k.shape[2], D, k.shape[1], P, int(q.dtype == torch.float16))
+        need = _work_bytes(dev, cu_kv is not None, key_mask is not None, sizes)
         work = torch.empty(need // 4, device=q.device, dtype=torch.float32) if need else None
-        a.work = native.ptr(work)
-        native.check(lib.tfb_context_attn(ctypes.byref(a), native.stream_ptr()), "tfb_context_attn")
+        args = _ARGS.pack(
+            qp, kk, vv, pre[0], pre[1], out.data_ptr(), native.ptr(lse) or 0, native.ptr(kv_lens) or 0, native.ptr(cu_kv) or 0,
+            native.ptr(key_mask) or 0, native.ptr(work) or 0, q_bs, q_ss, q_hs, k_bs, k_ss, k_hs, v_bs, v_ss, v_hs, *pre[2:],
+            key_mask.stride(0) if key_mask is not None else 0, *sizes, scale, 0)  # fmt: skip
+        native.check(native.load().tfb_context_attn(args, native.stream_ptr()), "tfb_context_attn")
     return (out, lse) if return_lse else out
 
 

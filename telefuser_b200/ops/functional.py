@@ -1131,19 +1131,36 @@ def rmsnorm_gate_residual(res, y, weight=None, gate=None, eps=1e-6, tanh_gate=Tr
 
 
 def _row_table(t, B, rows, C):
-    """fp32 modulation table of 1, B or `rows` rows of C -> (tensor, row stride, rows of the activations per table row).
-    Slices of a wider table are used in place (their row stride is kept)."""
-    t = t.float()
+    """fp32 modulation table of 1, B or `rows` rows of C -> (tensor, address, row stride, rows of the activations per table
+    row). Slices of a wider table are used in place (their row stride is kept)."""
+    if t is None:
+        return None, None, 0, 1
+    if t.dtype != torch.float32:
+        t = t.float()
     n = t.numel() // C
     if t.shape[-1] != C or n not in (1, B, rows):
         raise ValueError(f"a modulation table of shape {tuple(t.shape)} does not fit {B} samples / {rows} rows of {C}")
+    at = t.data_ptr()
+    if t.is_contiguous() and at % 16 == 0:
+        return t, at, C, rows // n
     lead = [(m, st) for m, st in zip(t.shape[:-1], t.stride()[:-1]) if m > 1]
     if len(lead) > 1 and all(lead[i][1] == lead[i + 1][0] * lead[i + 1][1] for i in range(len(lead) - 1)):
         lead = [(n, lead[-1][1])]
     ld = lead[0][1] if lead else 0
-    if len(lead) > 1 or ld % 4 or t.stride(-1) != 1 or t.data_ptr() % 16:
+    if len(lead) > 1 or ld % 4 or t.stride(-1) != 1 or at % 16:
         t, ld = t.clone(memory_format=torch.contiguous_format), C
-    return t, ld, max(1, rows // n)
+    return t, t.data_ptr(), ld, rows // n
+
+
+def _row_matrix(t, rows, C):
+    """-> (tensor, address, row stride) of `rows` 16-byte aligned rows of C; views with regular rows are used in place."""
+    at = t.data_ptr()
+    if t.is_contiguous() and at % 16 == 0:
+        return t, at, C
+    t = t.reshape(rows, C)
+    ok = t.stride(1) == 1 and t.data_ptr() % 16 == 0 and (rows == 1 or t.stride(0) * t.element_size() % 16 == 0)
+    t = t if ok else t.clone(memory_format=torch.contiguous_format)
+    return t, t.data_ptr(), t.stride(0) if rows > 1 else C
 
 
 def rmsnorm_gate_residual_modulate(res, y, weight=None, gate=None, next_weight=None, shift=None, scale=None, eps=1e-6,
@@ -1180,20 +1197,11 @@ def rmsnorm_gate_residual_modulate(res, y, weight=None, gate=None, next_weight=N
         with torch.cuda.device(res.device):
             return rmsnorm_gate_residual_modulate(res, y, weight, gate, next_weight, shift, scale, eps, tanh_gate, post_norm)
     rows = res.numel() // C if C else 0
-    x, h = (torch.empty(res.shape, device=res.device, dtype=res.dtype) for _ in range(2))
+    x = torch.empty(res.shape, device=res.device, dtype=res.dtype)
+    h = torch.empty(res.shape, device=res.device, dtype=res.dtype)
     if rows == 0:
         return x, h
-
-    def matrix(t):
-        t = t.reshape(rows, C)
-        ok = (t.stride(1) == 1 or C == 1) and t.data_ptr() % 16 == 0 and (rows == 1 or t.stride(0) * t.element_size() % 16 == 0)
-        t = t if ok else t.clone(memory_format=torch.contiguous_format)
-        return t, t.stride(0) if rows > 1 else C
-
-    r2, ldr = matrix(res)
-    y2, ldy = matrix(y)
-    weights = [w for w in (weight, next_weight) if w is not None]
-    w_f32 = any(w.dtype != res.dtype for w in weights)
+    w_f32 = any(w is not None and w.dtype != res.dtype for w in (weight, next_weight))
 
     def vector(w):
         if w is None:
@@ -1201,13 +1209,17 @@ def rmsnorm_gate_residual_modulate(res, y, weight=None, gate=None, next_weight=N
         w = (w.float() if w_f32 else w).contiguous()
         return w if w.data_ptr() % 16 == 0 else w.clone()
 
-    w1, w2 = vector(weight), vector(next_weight)
-    B = res.shape[0] if res.dim() > 2 else 1
-    g, sh, sc = ((None, 0, 1) if t is None else _row_table(t, B, rows, C) for t in (gate, shift, scale))
+    res, res_at, ldr = _row_matrix(res, rows, C)
+    y, y_at, ldy = _row_matrix(y, rows, C)
+    weight, next_weight = vector(weight), vector(next_weight)
+    B = x.shape[0] if x.dim() > 2 else 1
+    gate, gate_at, ldg, rpg = _row_table(gate, B, rows, C)
+    shift, shift_at, lds, rps = _row_table(shift, B, rows, C)
+    scale, scale_at, ldc, rpc = _row_table(scale, B, rows, C)
     code = native.load().tfb_sandwich_norm(
-        r2.data_ptr(), ldr, y2.data_ptr(), ldy, x.data_ptr(), h.data_ptr(), rows, C, float(eps), _SNORM_TYPES[res.dtype],
-        int(w_f32), native.ptr(w1), native.ptr(w2), native.ptr(g[0]), g[1], g[2], native.ptr(sh[0]), sh[1], sh[2],
-        native.ptr(sc[0]), sc[1], sc[2], int(post_norm), int(tanh_gate), native.stream_ptr())  # fmt: skip
+        res_at, ldr, y_at, ldy, x.data_ptr(), h.data_ptr(), rows, C, eps, _SNORM_TYPES[x.dtype], w_f32, native.ptr(weight),
+        native.ptr(next_weight), gate_at, ldg, rpg, shift_at, lds, rps, scale_at, ldc, rpc, post_norm, tanh_gate,
+        native.stream_ptr())  # fmt: skip
     native.check(code, "tfb_sandwich_norm")
     return x, h
 

@@ -20,6 +20,7 @@ _LOCK = threading.Lock()
 _LAUNCHES = 0  # number of native kernel launches issued through this module
 
 c_void_p = ctypes.c_void_p
+c_char_p = ctypes.c_char_p
 c_int = ctypes.c_int
 c_long = ctypes.c_long
 c_float = ctypes.c_float
@@ -138,7 +139,7 @@ def _declare(lib) -> None:
                              c_int, c_int, c_void_p, c_int, c_void_p],
         "tfb_slab_reduce": [c_void_p, c_int, c_long, c_int, c_long, c_void_p, c_void_p, c_long, c_void_p, c_long, c_int,
                             c_long, c_void_p, c_int, c_long, c_long, c_void_p],
-        "tfb_context_attn": [c_void_p, c_void_p],
+        "tfb_context_attn": [c_char_p, c_void_p],  # tfb_context_attn_args, packed
         "tfb_sandwich_norm": [c_void_p, c_long, c_void_p, c_long, c_void_p, c_void_p, c_long, c_int, c_float, c_int, c_int,
                               c_void_p, c_void_p, c_void_p, c_long, c_long, c_void_p, c_long, c_long, c_void_p, c_long,
                               c_long, c_int, c_int, c_void_p],
@@ -146,7 +147,7 @@ def _declare(lib) -> None:
                               c_int, c_int, c_int, c_long, c_long, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p],
     }  # fmt: skip
     lib.tfb_context_attn_work.restype = c_long
-    lib.tfb_context_attn_work.argtypes = [c_void_p]
+    lib.tfb_context_attn_work.argtypes = [c_char_p]
     for name, args in table.items():
         fn = getattr(lib, name)
         fn.restype = c_int
@@ -186,7 +187,7 @@ def use_native(t: torch.Tensor) -> bool:
 
 
 def stream_ptr() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def check(code: int, what: str) -> None:
