@@ -44,7 +44,19 @@ __device__ __forceinline__ uint32_t ctx_pack2(float lo, float hi) {
   return FP16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
 }
 
-// Few query rows (Sq * H / Hkv <= 16) of every sample against its own keys.
+// [batch][token][head][channel] tensor map; a dimension of one entry may have any stride (TMA wants multiples of 16).
+inline int ctx_tmap(CUtensorMap* m, const void* base, int fp16, int D, int heads, long hs, long rows, long ss, int B, long bs,
+                    uint32_t box_c, uint32_t box_h, uint32_t box_s, int swizzle) {
+  uint64_t dims[4] = {static_cast<uint64_t>(D), static_cast<uint64_t>(heads), static_cast<uint64_t>(rows),
+                      static_cast<uint64_t>(B)};
+  uint64_t str[3] = {static_cast<uint64_t>(heads > 1 ? hs : 8) * 2, static_cast<uint64_t>(rows > 1 ? ss : 8) * 2,
+                     static_cast<uint64_t>(B > 1 ? bs : 8) * 2};
+  uint32_t box[4] = {box_c, box_h, box_s, 1};
+  return make_tmap(m, base, fp16 ? TM_F16 : TM_BF16, 4, dims, str, box, swizzle);
+}
+
+// Few query rows (Sq * H / Hkv <= CTX_FEW_ROWS) of every sample against its own keys.
+constexpr int CTX_FEW_ROWS = 32;
 int launch_ctx_rows(const CtxParams& p, int fp16, cudaStream_t st);
 // Joins p.ns slots of part_o / part_lse (slot0 = 0) into out and lse.
 int launch_ctx_join(const CtxParams& p, int fp16, cudaStream_t st);

@@ -1,6 +1,6 @@
 // C entry points of context attention: argument checks, the choice of kernels and key splits.
 //
-// Rows kernel (context_attn_rows.cu) when a sample has at most 16 query rows per key head, tensor-memory kernel
+// Rows kernel (context_attn_rows.cu) when a sample has at most 32 query rows per key head, tensor-memory kernel
 // (context_attn_tc.cu) otherwise. A shared prefix is visited by the tensor-memory kernel as the first key blocks of every
 // sample when the sample fills a query tile; below that the prefix is computed once for all samples - their tokens form
 // one batch entry - as slots of its own, the samples' own keys as further slots, and the join adds them up.
@@ -19,14 +19,14 @@ struct CtxPlan {
   int slots() const { return (apart ? ns_prefix : 0) + ns; }
 };
 
-bool few_rows(long tokens, int H, int Hkv) { return tokens * (H / Hkv) <= 16; }
+bool few_rows(long tokens, int H, int Hkv) { return tokens * (H / Hkv) <= CTX_FEW_ROWS; }
 
-// Splits of the key range so that few items still fill the device: about three CTAs per SM for the rows kernel (three
-// are resident), one per SM for the tensor-memory kernel; a slice is never shorter than what a CTA takes in one step.
+// Splits of the key range so that few items still fill the device: two CTAs per SM for the rows kernel (two are
+// resident), one per SM for the tensor-memory kernel; a slice is never shorter than what a CTA takes in one step.
 int pick_splits(bool rows, int B, long Sq, int H, int Hkv, long keys) {
   const long sms = sm_count();
   const long items = rows ? static_cast<long>(B) * Hkv : ctx_tc_items(B, static_cast<int>(Sq), H, Hkv);
-  long ns = (rows ? 3 * sms : sms) / (items > 0 ? items : 1);
+  long ns = (rows ? 2 * sms : sms) / (items > 0 ? items : 1);
   const long most = (keys + 127) / 128 / (rows ? 1 : 2);
   if (ns > most) ns = most;
   if (ns > CTX_MAX_SPLITS) ns = CTX_MAX_SPLITS;

@@ -1,51 +1,84 @@
 // Context attention for a few query rows (single tokens, a handful of summary tokens): memory bound, every key and
 // value row is read once per (sample, key head).
 //
-// One CTA of four warps owns the <= 16 query rows of one (sample, key head) - tokens x grouped heads - and one slice of
-// the keys; its warps take 16 keys at a time and keep their own running maximum, sum and 16 x D fp32 accumulator, joined
-// once at the end through shared memory. The products run on mma.sync m16n8k16: with at most 16 rows the tensor work is
-// 1/8 of what the loads take, and operands go from global memory to registers without a stop in shared memory. For
-// that the fragment layouts are met by permuting the summation index instead of the data:
-//   Q.K^T  lane (n = lane / 4, c = lane % 4) loads 16 bytes of key n, channels 32 i + 8 c .. + 7: two k16 steps whose
-//          channel order is permuted the same way in Q and K.
-//   P.V    lane loads 16 bytes (channels 64 i + 8 n .. + 7) of the keys 2c, 2c + 1, 2c + 8, 2c + 9, the keys its P fragment
-//          holds; byte permutes pair two keys per register. Column n of MMA t is channel 64 i + 8 n + t.
-// Rows that the lengths or the mask hide are not loaded at all: zeros take their place, so infinities and NaN there
-// never meet a product, and their scores are replaced by -inf.
+// One CTA of four warps owns the <= 32 query rows of one (sample, key head) - tokens x grouped heads - and one slice of the
+// keys. Its warps work for themselves, 16 keys at a time: a warp has a ring of TMA boxes in shared memory (K and V of 16 keys
+// each), its own running maximum, sum and fp32 accumulator, and refills a slot as soon as it has read it; the four results
+// are joined once at the end. So bytes in flight cost no registers: two CTAs per SM hold about 180 KB of the stream, and no
+// warp waits for another. The products run on mma.sync m16n8k16, fed by ldmatrix: with so few rows the tensor work is a
+// fraction of what the loads take.
+// Keys that the length or the mask hides: their scores are replaced by -inf and their V fragments by zeros, so infinities
+// and NaN there never meet a product.
 //
 // Bound by HBM where the batch fills the device, by launch and load latency below that.
+#include <string.h>
+
 #include "context_attn.cuh"
 
 namespace tfb {
 
 constexpr int CR_WARPS = 4;
 
+struct CtxRowsParams {
+  CtxParams c;
+  int bmul;  // 0: packed samples, the tensors have one batch entry
+};
+
 template <bool FP16>
-__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if (FP16)
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// Byte offset of the 16-byte piece `piece` of row `row` in boxes of [16 rows][64 channels], 128B swizzle, 2 KB each.
+__device__ __forceinline__ uint32_t box_at(int row, int piece) {
+  return (piece >> 3) * 2048 + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
 }
 
-__device__ __forceinline__ uint4 ctx_ld16(const uint16_t* p, bool ok) {
-  uint4 r = make_uint4(0, 0, 0, 0);
-  if (ok) r = __ldg(reinterpret_cast<const uint4*>(p));
-  return r;
-}
+template <int DK, int MT>
+struct CtxRowsCfg {
+  static constexpr int CHUNK = 2 * 16 * DK * 2;             // K and V of 16 keys
+  static constexpr int STAGES = DK == 128 ? 3 : 6;          // per warp: 24 KB in flight
+  static constexpr int RING = CR_WARPS * STAGES * CHUNK;    // 96 KB; the join at the end lies over it
+  static constexpr int Q_OFF = RING;                        // MT x 16 rows as boxes
+  static constexpr int ML_OFF = Q_OFF + MT * 16 * DK * 2;   // [warps][MT * 16] of (maximum, sum)
+  static constexpr int BAR_OFF = ML_OFF + CR_WARPS * MT * 16 * 8;
+  static constexpr int SMEM = BAR_OFF + CR_WARPS * STAGES * 8 + 16 + 1024;
+  static_assert(CR_WARPS * MT * 16 * DK * 4 <= RING, "the join fits over the ring");
+  static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs per SM");
+};
 
-template <bool FP16, int DK>
-__global__ void __launch_bounds__(CR_WARPS * 32) ctx_rows_kernel(const CtxParams p) {
-  constexpr int NCH = DK / 32, NBLK = DK / 64;
-  __shared__ float s_o[CR_WARPS][16][DK];
-  __shared__ float s_m[CR_WARPS][16], s_l[CR_WARPS][16];
+template <bool FP16, int DK, int MT>
+__global__ void __launch_bounds__(CR_WARPS * 32, 2)
+    ctx_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                    const __grid_constant__ CtxRowsParams rp) {
+  using Cfg = CtxRowsCfg<DK, MT>;
+  constexpr int NBOX = DK / 64, ROWS = MT * 16;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const CtxParams& p = rp.c;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::BAR_OFF);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + CR_WARPS * Cfg::STAGES);
+  const AbortCtx ctx{abort_flag, p.status};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n = lane >> 2, c = lane & 3;
+  const int c = lane & 3;
   const int G = p.H / p.Hkv, R = p.Sq * G;
   const int split = blockIdx.x % p.ns;
   const int hk = (blockIdx.x / p.ns) % p.Hkv;
@@ -55,150 +88,173 @@ __global__ void __launch_bounds__(CR_WARPS * 32) ctx_rows_kernel(const CtxParams
   const long n16 = (len + 15) >> 4;
   const int i0 = static_cast<int>(n16 * split / p.ns), i1 = static_cast<int>(n16 * (split + 1) / p.ns);
 
-  const uint16_t* qb = static_cast<const uint16_t*>(p.q) + static_cast<long>(b) * p.q_bs;
-  const uint16_t* kb = static_cast<const uint16_t*>(p.k) + (p.cu_kv ? 0 : static_cast<long>(b) * p.k_bs) +
-                       static_cast<long>(first) * p.k_ss + static_cast<long>(hk) * p.k_hs;
-  const uint16_t* vb = static_cast<const uint16_t*>(p.v) + (p.cu_kv ? 0 : static_cast<long>(b) * p.v_bs) +
-                       static_cast<long>(first) * p.v_ss + static_cast<long>(hk) * p.v_hs;
-  const uint8_t* mb = p.key_mask ? p.key_mask + static_cast<long>(b) * p.mask_bs : nullptr;
-  auto visible = [&](int j) { return j < len && (!mb || mb[j]); };
-
-  uint4 q0[NCH], q1[NCH];
+  uint64_t* full = bars + warp * Cfg::STAGES;
+  uint8_t* ring = smem + warp * Cfg::STAGES * Cfg::CHUNK;
+  // one lane: K and V of the 16 keys of chunk `it`
+  auto fetch = [&](int it, int slot) {
+    uint8_t* dst = ring + slot * Cfg::CHUNK;
+    mbar_expect_tx(&full[slot], Cfg::CHUNK);
 #pragma unroll
-  for (int i = 0; i < NCH; ++i) {
-    const int d = i * 32 + c * 8;
-    const int ra = n, rb = n + 8;
-    q0[i] = ctx_ld16(qb + (ra / G) * p.q_ss + static_cast<long>(hk * G + ra % G) * p.q_hs + d, ra < R && d < p.D);
-    q1[i] = ctx_ld16(qb + (rb / G) * p.q_ss + static_cast<long>(hk * G + rb % G) * p.q_hs + d, rb < R && d < p.D);
-  }
-  float o[NBLK][8][4];
-#pragma unroll
-  for (int i = 0; i < NBLK; ++i)
-#pragma unroll
-    for (int t = 0; t < 8; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][t][e] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-
-  uint4 kf[2][NCH];
-  auto load_k = [&](int it) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int j = it * 16 + t * 8 + n;
-      const bool ok = it < i1 && visible(j);
-#pragma unroll
-      for (int i = 0; i < NCH; ++i) {
-        const int d = i * 32 + c * 8;
-        kf[t][i] = ctx_ld16(kb + static_cast<long>(j) * p.k_ss + d, ok && d < p.D);
-      }
+    for (int x = 0; x < NBOX; ++x) {
+      tma_load_4d(dst + x * 2048, &tmK, &full[slot], x * 64, hk, first + it * 16, b * rp.bmul);
+      tma_load_4d(dst + (NBOX + x) * 2048, &tmV, &full[slot], x * 64, hk, first + it * 16, b * rp.bmul);
     }
   };
-  load_k(i0 + warp);
-  for (int it = i0 + warp; it < i1; it += CR_WARPS) {
-    const int j0 = it * 16;
-    bool vis[4];
-    uint4 vf[4][NBLK];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int j = j0 + 2 * c + (e & 1) + (e >> 1) * 8;
-      vis[e] = visible(j);
-#pragma unroll
-      for (int i = 0; i < NBLK; ++i) {
-        const int d = i * 64 + n * 8;
-        vf[e][i] = ctx_ld16(vb + static_cast<long>(j) * p.v_ss + d, vis[e] && d < p.D);
-      }
+  if (lane == 0) {
+    for (int s = 0; s < Cfg::STAGES; ++s) mbar_init(&full[s], 1);
+    mbar_fence_init();
+    for (int s = 0; s < Cfg::STAGES; ++s) {
+      const int it = i0 + warp + s * CR_WARPS;
+      if (it < i1) fetch(it, s);
     }
-    float s[2][4];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[t][e] = 0.f;
-#pragma unroll
-      for (int i = 0; i < NCH; ++i) {
-        mma16816<FP16>(s[t], q0[i].x, q1[i].x, q0[i].y, q1[i].y, kf[t][i].x, kf[t][i].y);
-        mma16816<FP16>(s[t], q0[i].z, q1[i].z, q0[i].w, q1[i].w, kf[t][i].z, kf[t][i].w);
-      }
-    }
-    load_k(it + CR_WARPS);
-    // s[t][0..1]: row n, keys 8 t + 2 c + {0, 1}; s[t][2..3]: row n + 8
-    float pr[2][4];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          s[t][r * 2 + e] = vis[t * 2 + e] ? s[t][r * 2 + e] * p.scale_log2 : -INFINITY;
-          mx = fmaxf(mx, s[t][r * 2 + e]);
-        }
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float m_new = fmaxf(m[r], mx);
-      if (__any_sync(0xffffffffu, m_new > m[r])) {
-        const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m[r] - m_new);
-        l[r] *= alpha;
-#pragma unroll
-        for (int i = 0; i < NBLK; ++i)
-#pragma unroll
-          for (int t = 0; t < 8; ++t) o[i][t][r * 2] *= alpha, o[i][t][r * 2 + 1] *= alpha;
-        m[r] = m_new;
-      }
-      const float base = m[r] == -INFINITY ? 0.f : m[r];
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          pr[t][r * 2 + e] = fast_exp2(s[t][r * 2 + e] - base);
-          l[r] += pr[t][r * 2 + e];
-        }
-    }
-    // P enters the product in the inputs' type (values in [0, 1]); its sum stays in fp32
-    const uint32_t a0 = ctx_pack2<FP16>(pr[0][0], pr[0][1]), a1 = ctx_pack2<FP16>(pr[0][2], pr[0][3]);
-    const uint32_t a2 = ctx_pack2<FP16>(pr[1][0], pr[1][1]), a3 = ctx_pack2<FP16>(pr[1][2], pr[1][3]);
-#pragma unroll
-    for (int i = 0; i < NBLK; ++i) {
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const uint32_t k0 = (&vf[0][i].x)[w], k1 = (&vf[1][i].x)[w], k8 = (&vf[2][i].x)[w], k9 = (&vf[3][i].x)[w];
-        mma16816<FP16>(o[i][2 * w], a0, a1, a2, a3, __byte_perm(k0, k1, 0x5410), __byte_perm(k8, k9, 0x5410));
-        mma16816<FP16>(o[i][2 * w + 1], a0, a1, a2, a3, __byte_perm(k0, k1, 0x7632), __byte_perm(k8, k9, 0x7632));
-      }
-    }
+    if (warp == 0) *abort_flag = 0;
   }
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    const int row = n + r * 8;
-    if (c == 0) s_m[warp][row] = m[r], s_l[warp][row] = l[r];
-    // column 2c of MMA t is channel 64 i + 16 c + t, column 2c + 1 the channel 8 further
-    if (row < R) {
-#pragma unroll
-      for (int i = 0; i < NBLK; ++i)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int t = 0; t < 8; t += 4)
-            *reinterpret_cast<float4*>(&s_o[warp][row][i * 64 + c * 16 + e * 8 + t]) =
-                make_float4(o[i][t][r * 2 + e], o[i][t + 1][r * 2 + e], o[i][t + 2][r * 2 + e], o[i][t + 3][r * 2 + e]);
-    }
+  // Q rows (token, head) as boxes, zeros behind the last
+  for (int x = threadIdx.x; x < ROWS * DK / 8; x += CR_WARPS * 32) {
+    const int row = x / (DK / 8), piece = x % (DK / 8);
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (row < R && piece * 8 < p.D)
+      v = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + static_cast<long>(b) * p.q_bs +
+                                               (row / G) * p.q_ss + static_cast<long>(hk * G + row % G) * p.q_hs + piece * 8));
+    *reinterpret_cast<uint4*>(smem + Cfg::Q_OFF + (row >> 4) * (16 * DK * 2) + box_at(row & 15, piece)) = v;
   }
   __syncthreads();
+
+  float o[MT][DK / 8][4];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int t = 0; t < DK / 8; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[mt][t][e] = 0.f;
+  float m[MT][2], l[MT][2];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) m[mt][0] = m[mt][1] = -INFINITY, l[mt][0] = l[mt][1] = 0.f;
+
+  const uint8_t* mb = p.key_mask ? p.key_mask + static_cast<long>(b) * p.mask_bs : nullptr;
+  const uint32_t q_at = smem_u32(smem + Cfg::Q_OFF);
+  // ldmatrix rows of this lane: A fragments and V take rows 0..15 by halves of a k-step, K takes the two key octets
+  const int a_row = lane & 15, a_half = lane >> 4;
+  const int k_row = (lane & 7) + ((lane >> 4) << 3), k_half = (lane >> 3) & 1;
+  int slot = 0;
+  uint32_t phase = 0;
+  for (int it = i0 + warp; it < i1; it += CR_WARPS) {
+    // keys of this lane's score columns: 2c, 2c + 1, 2c + 8, 2c + 9 of the chunk
+    bool vis[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int j = it * 16 + 2 * c + (e & 1) + (e >> 1) * 8;
+      vis[e] = j < len && (!mb || mb[j]);
+    }
+    // after an expired wait (recorded in the status word) the warp goes on with what is there, to the common end
+    mbar_wait_warp(&full[slot], phase, ctx, 80);
+    const uint32_t k_at = smem_u32(ring + slot * Cfg::CHUNK), v_at = k_at + NBOX * 2048;
+    float s[MT][2][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[mt][t][e] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < DK / 16; ++kk) {
+      uint32_t kf[4];
+      ldsm4(k_at + box_at(k_row, kk * 2 + k_half), kf);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        uint32_t a[4];
+        ldsm4(q_at + mt * (16 * DK * 2) + box_at(a_row, kk * 2 + a_half), a);
+        mma16816<FP16>(s[mt][0], a, kf[0], kf[1]);
+        mma16816<FP16>(s[mt][1], a, kf[2], kf[3]);
+      }
+    }
+    uint32_t pf[MT][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float& v = s[mt][t][r * 2 + e];
+            v = vis[t * 2 + e] ? v * p.scale_log2 : -INFINITY;
+            mx = fmaxf(mx, v);
+          }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float m_new = fmaxf(m[mt][r], mx);
+        if (__any_sync(0xffffffffu, m_new > m[mt][r])) {
+          const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m[mt][r] - m_new);
+          l[mt][r] *= alpha;
+#pragma unroll
+          for (int t = 0; t < DK / 8; ++t) o[mt][t][r * 2] *= alpha, o[mt][t][r * 2 + 1] *= alpha;
+          m[mt][r] = m_new;
+        }
+        const float base = m[mt][r] == -INFINITY ? 0.f : m[mt][r];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const float p0 = fast_exp2(s[mt][t][r * 2] - base), p1 = fast_exp2(s[mt][t][r * 2 + 1] - base);
+          l[mt][r] += p0 + p1;
+          pf[mt][t * 2 + r] = ctx_pack2<FP16>(p0, p1);  // in [0, 1], rounded to the inputs' type for the product
+        }
+      }
+    }
+    const bool all = __all_sync(0xffffffffu, vis[0] && vis[1] && vis[2] && vis[3]);
+    const uint32_t keep0 = (vis[0] ? 0xffffu : 0u) | (vis[1] ? 0xffff0000u : 0u);
+    const uint32_t keep1 = (vis[2] ? 0xffffu : 0u) | (vis[3] ? 0xffff0000u : 0u);
+#pragma unroll
+    for (int t = 0; t < DK / 16; ++t) {
+      uint32_t vf[4];  // keys 0..7 / 8..15 of channels 16 t .. + 7, then of the next 8
+      ldsm4_t(v_at + box_at(a_row, t * 2 + a_half), vf);
+      if (!all) vf[0] &= keep0, vf[1] &= keep1, vf[2] &= keep0, vf[3] &= keep1;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        mma16816<FP16>(o[mt][2 * t], pf[mt], vf[0], vf[1]);
+        mma16816<FP16>(o[mt][2 * t + 1], pf[mt], vf[2], vf[3]);
+      }
+    }
+    __syncwarp();
+    if (lane == 0 && it + Cfg::STAGES * CR_WARPS < i1) fetch(it + Cfg::STAGES * CR_WARPS, slot);
+    if (++slot == Cfg::STAGES) slot = 0, phase ^= 1;
+  }
+
+  // ---- join of the four warps, over the rings (every copy that was issued has been waited for) ----
+  __syncthreads();
+  float* s_o = reinterpret_cast<float*>(smem) + warp * ROWS * DK;
+  float2* s_ml = reinterpret_cast<float2*>(smem + Cfg::ML_OFF);
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float sum = l[mt][r];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      const int row = mt * 16 + (lane >> 2) + r * 8;
+      if (c == 0) s_ml[warp * ROWS + row] = make_float2(m[mt][r], sum);
+      if (row < R)
+#pragma unroll
+        for (int t = 0; t < DK / 8; ++t)
+          *reinterpret_cast<float2*>(s_o + row * DK + t * 8 + 2 * c) = make_float2(o[mt][t][r * 2], o[mt][t][r * 2 + 1]);
+    }
+  __syncthreads();
+  s_o = reinterpret_cast<float*>(smem);
   const int per_row = p.D >> 2;  // float4 groups of a row
   for (int x = threadIdx.x; x < R * per_row; x += CR_WARPS * 32) {
     const int row = x / per_row, d = (x - row * per_row) * 4;
-    float mm = s_m[0][row];
+    float mm = s_ml[row].x;
 #pragma unroll
-    for (int w = 1; w < CR_WARPS; ++w) mm = fmaxf(mm, s_m[w][row]);
+    for (int w = 1; w < CR_WARPS; ++w) mm = fmaxf(mm, s_ml[w * ROWS + row].x);
     const float base = mm == -INFINITY ? 0.f : mm;
     float sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < CR_WARPS; ++w) {
-      const float f = fast_exp2(s_m[w][row] - base);
-      sum += f * s_l[w][row];
-      const float4 t = *reinterpret_cast<const float4*>(&s_o[w][row][d]);
+      const float2 ml = s_ml[w * ROWS + row];
+      const float f = fast_exp2(ml.x - base);
+      sum += f * ml.y;
+      const float4 t = *reinterpret_cast<const float4*>(s_o + (w * ROWS + row) * DK + d);
       acc.x += f * t.x, acc.y += f * t.y, acc.z += f * t.z, acc.w += f * t.w;
     }
     const float inv = sum > 0.f ? 1.f / sum : 0.f;
@@ -219,29 +275,39 @@ __global__ void __launch_bounds__(CR_WARPS * 32) ctx_rows_kernel(const CtxParams
   }
 }
 
-// out = sum_s w_s o_s / sum_s w_s, w_s = 2^(lse_s - max): one warp per (token, head), slots added in their order.
+// out = sum_s w_s o_s / sum_s w_s, w_s = 2^(lse_s - max). One CTA of four warps per (token, head): a warp adds every fourth
+// slot, in an order that depends on nothing but the number of slots.
 template <bool FP16>
-__global__ void __launch_bounds__(256) ctx_join_kernel(const CtxParams p) {
+__global__ void __launch_bounds__(128) ctx_join_kernel(const CtxParams p) {
+  __shared__ float4 s_acc[4][32];
+  __shared__ float s_sum[4];
   const long rows = static_cast<long>(p.B) * p.Sq * p.H;
-  const long row = blockIdx.x * 8L + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (row >= rows) return;
+  const long row = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float mm = -INFINITY;
   for (int s = lane; s < p.ns; s += 32) mm = fmaxf(mm, p.part_lse[s * rows + row]);
   mm = warp_max(mm);
+  const float base = mm == -INFINITY ? 0.f : mm;
   float sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   const int d = lane * 4;
 #pragma unroll 4
-  for (int s = 0; s < p.ns; ++s) {
-    const float ls = p.part_lse[s * rows + row];
-    if (ls == -INFINITY) continue;
-    const float f = fast_exp2(ls - mm);
+  for (int s = warp; s < p.ns; s += 4) {
+    const float f = fast_exp2(p.part_lse[s * rows + row] - base);  // 0 for a slot that saw no key: its part_o holds nothing
+    float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (d < p.D && f > 0.f) t = *reinterpret_cast<const float4*>(p.part_o + (s * rows + row) * p.D + d);
     sum += f;
-    if (d < p.D) {
-      const float4 t = *reinterpret_cast<const float4*>(p.part_o + (s * rows + row) * p.D + d);
-      acc.x += f * t.x, acc.y += f * t.y, acc.z += f * t.z, acc.w += f * t.w;
-    }
+    acc.x += f * t.x, acc.y += f * t.y, acc.z += f * t.z, acc.w += f * t.w;
+  }
+  s_acc[warp][lane] = acc;
+  if (lane == 0) s_sum[warp] = sum;
+  __syncthreads();
+  if (warp) return;
+#pragma unroll
+  for (int w = 1; w < 4; ++w) {
+    const float4 t = s_acc[w][lane];
+    acc.x += t.x, acc.y += t.y, acc.z += t.z, acc.w += t.w;
+    sum += s_sum[w];
   }
   const float inv = sum > 0.f ? 1.f / sum : 0.f;
   if (d < p.D)
@@ -255,25 +321,48 @@ __global__ void __launch_bounds__(256) ctx_join_kernel(const CtxParams p) {
   }
 }
 
-int launch_ctx_rows(const CtxParams& p, int fp16, cudaStream_t st) {
+template <bool FP16, int DK, int MT>
+static int launch_ctx_rows_impl(const CtxParams& p, cudaStream_t st) {
+  using Cfg = CtxRowsCfg<DK, MT>;
+  static bool attr_set[TFB_MAX_DEVICES] = {false};
+  auto kern = &ctx_rows_kernel<FP16, DK, MT>;
+  if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), Cfg::SMEM, attr_set)) return rc;
   const long ctas = static_cast<long>(p.B) * p.Hkv * p.ns;
-  if (p.Sq * (p.H / p.Hkv) > 16 || ctas > 0x7fffffffL) return TFB_ERR_TOO_LARGE;
-  const int g = static_cast<int>(ctas);
-  if (p.D <= 64) {
-    if (fp16) ctx_rows_kernel<true, 64><<<g, CR_WARPS * 32, 0, st>>>(p);
-    else ctx_rows_kernel<false, 64><<<g, CR_WARPS * 32, 0, st>>>(p);
-  } else {
-    if (fp16) ctx_rows_kernel<true, 128><<<g, CR_WARPS * 32, 0, st>>>(p);
-    else ctx_rows_kernel<false, 128><<<g, CR_WARPS * 32, 0, st>>>(p);
+  if (ctas > 0x7fffffffL) return TFB_ERR_TOO_LARGE;
+  CtxRowsParams rp;
+  rp.c = p;
+  rp.bmul = p.cu_kv ? 0 : 1;
+  CUtensorMap tk, tv;
+  if (p.Skv > 0) {
+    const int kb = p.cu_kv ? 1 : p.B;
+    int e;
+    if ((e = ctx_tmap(&tk, p.k, FP16, p.D, p.Hkv, p.k_hs, p.Skv, p.k_ss, kb, p.k_bs, 64, 1, 16, TM_SW_128))) return e;
+    if ((e = ctx_tmap(&tv, p.v, FP16, p.D, p.Hkv, p.v_hs, p.Skv, p.v_ss, kb, p.v_bs, 64, 1, 16, TM_SW_128))) return e;
+  } else {  // no keys at all: the maps are not used
+    memset(&tk, 0, sizeof(tk));
+    memset(&tv, 0, sizeof(tv));
   }
+  kern<<<static_cast<int>(ctas), CR_WARPS * 32, Cfg::SMEM, st>>>(tk, tv, rp);
   return cudaGetLastError() == cudaSuccess ? TFB_OK : TFB_ERR_LAUNCH;
 }
 
+template <bool FP16>
+static int launch_ctx_rows_type(const CtxParams& p, cudaStream_t st) {
+  const bool one = p.Sq * (p.H / p.Hkv) <= 16;
+  if (p.D <= 64) return one ? launch_ctx_rows_impl<FP16, 64, 1>(p, st) : launch_ctx_rows_impl<FP16, 64, 2>(p, st);
+  return one ? launch_ctx_rows_impl<FP16, 128, 1>(p, st) : launch_ctx_rows_impl<FP16, 128, 2>(p, st);
+}
+
+int launch_ctx_rows(const CtxParams& p, int fp16, cudaStream_t st) {
+  if (static_cast<long>(p.Sq) * (p.H / p.Hkv) > CTX_FEW_ROWS) return TFB_ERR_TOO_LARGE;
+  return fp16 ? launch_ctx_rows_type<true>(p, st) : launch_ctx_rows_type<false>(p, st);
+}
+
 int launch_ctx_join(const CtxParams& p, int fp16, cudaStream_t st) {
-  const long blocks = (static_cast<long>(p.B) * p.Sq * p.H + 7) / 8;
-  if (blocks > 0x7fffffffL) return TFB_ERR_TOO_LARGE;
-  if (fp16) ctx_join_kernel<true><<<static_cast<int>(blocks), 256, 0, st>>>(p);
-  else ctx_join_kernel<false><<<static_cast<int>(blocks), 256, 0, st>>>(p);
+  const long rows = static_cast<long>(p.B) * p.Sq * p.H;
+  if (rows > 0x7fffffffL) return TFB_ERR_TOO_LARGE;
+  if (fp16) ctx_join_kernel<true><<<static_cast<int>(rows), 128, 0, st>>>(p);
+  else ctx_join_kernel<false><<<static_cast<int>(rows), 128, 0, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? TFB_OK : TFB_ERR_LAUNCH;
 }
 

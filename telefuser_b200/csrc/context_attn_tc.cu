@@ -62,7 +62,35 @@ struct CtxItem {
   __device__ __forceinline__ bool two(const CtxTcParams& p) const { return (qp * 2 + 1) * p.tok < p.c.Sq; }
 };
 
-__device__ __forceinline__ CtxItem ctx_item(const CtxTcParams& p, int i) {
+// First visible key of mask[0, n) and one past the last (n, 0 if there is none). Whole warp; reads from both ends inwards,
+// so what lies between the ends is not read.
+__device__ __forceinline__ void ctx_mask_ends(const uint8_t* mask, int n, int& lo, int& hi) {
+  constexpr int STEP = 16;  // loads in flight per lane
+  lo = n;
+  hi = 0;
+  for (int at = 0; at < n && lo == n; at += 32 * STEP) {
+    int found = n;
+#pragma unroll
+    for (int x = 0; x < STEP; ++x) {
+      const int j = at + x * 32 + static_cast<int>(lane_id());
+      if (j < n && __ldg(mask + j)) found = min(found, j);
+    }
+    lo = __reduce_min_sync(0xffffffffu, found);
+  }
+  for (int at = n; at > lo && hi == 0; at -= 32 * STEP) {
+    int found = 0;
+#pragma unroll
+    for (int x = 0; x < STEP; ++x) {
+      const int j = at - 1 - (x * 32 + static_cast<int>(lane_id()));
+      if (j >= lo && __ldg(mask + j)) found = max(found, j + 1);
+    }
+    hi = __reduce_max_sync(0xffffffffu, found);
+  }
+}
+
+// Work item i; `ends` holds what the mask leaves of sample ends_b. Whole warp.
+template <bool MASK>
+__device__ __forceinline__ CtxItem ctx_item(const CtxTcParams& p, int i, int& ends_b, int2& ends) {
   CtxItem t;
   t.qp = i % p.n_qp;
   i /= p.n_qp;
@@ -71,9 +99,20 @@ __device__ __forceinline__ CtxItem ctx_item(const CtxTcParams& p, int i) {
   t.hg = i % p.n_hg;
   t.b = i / p.n_hg;
   ctx_sample_range(p.c, t.b, t.first, t.len);
-  const long nb = p.n_prefix + ((t.len + 127) >> 7);
-  t.j0 = static_cast<int>(nb * t.split / p.c.ns);
-  t.nb = static_cast<int>(nb * (t.split + 1) / p.c.ns) - t.j0;
+  int skip = 0;  // blocks in front of the first visible key
+  if (MASK) {
+    if (t.b != ends_b) ctx_mask_ends(p.c.key_mask + static_cast<long>(t.b) * p.c.mask_bs, t.len, ends.x, ends.y);
+    ends_b = t.b;
+    t.len = ends.y;
+    skip = t.len > 0 ? ends.x >> 7 : 0;
+  }
+  const int nb = p.n_prefix + ((t.len + 127) >> 7) - skip;
+  if (p.c.ns == 1) {
+    t.j0 = skip, t.nb = nb;
+  } else {
+    t.j0 = skip + static_cast<int>(static_cast<long>(nb) * t.split / p.c.ns);
+    t.nb = skip + static_cast<int>(static_cast<long>(nb) * (t.split + 1) / p.c.ns) - t.j0;
+  }
   return t;
 }
 // Visible keys of block j, at most 128 (before the mask).
@@ -290,6 +329,7 @@ __global__ void __launch_bounds__(512, 1)
     uint8_t* stage = smem + CT_OUT_OFF + wq * 8192;
     const int row_tok = row / p.pack, row_head = row % p.pack;
     uint32_t o_phase = 0;  // bit per query tile
+    int n_box = 0;
     bool ok = true;
     while (ok && items.next(t, ctx, 55)) {
       for (int st = 0; st < (t.two(p) ? 2 : 1); ++st) {
@@ -329,37 +369,37 @@ __global__ void __launch_bounds__(512, 1)
         } else {
           if (p.c.lse && row_ok)
             p.c.lse[(static_cast<long>(t.b) * p.c.H + head) * p.c.Sq + tok] = lse2 * 0.6931471805599453f;
-          if (lane == 0) tma_store_wait_read0();  // the boxes of the previous tile have left
-          __syncwarp();
           const int first_tok = tile_tok + wq * 32 / p.pack;
 #pragma unroll
           for (int x = 0; x < NBOX; ++x) {
             if (x * 64 < p.c.D) {
-              uint8_t* buf = stage + x * 4096 + lane * 128;
+              if (lane == 0) tma_store_wait_read1();  // the box before the last has left this buffer
+              __syncwarp();
+              uint8_t* buf = stage + (n_box++ & 1) * 4096;
 #pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                uint32_t o[16];
+              for (int c = 0; c < 2; ++c) {
+                uint32_t o[32];
                 if (t.nb > 0) {
-                  tmem_ld_32x16(tmem_o + x * 64 + c * 16, o);
+                  tmem_ld_32x32(tmem_o + x * 64 + c * 32, o);
                   tmem_ld_wait();
                 } else {
 #pragma unroll
-                  for (int e = 0; e < 16; ++e) o[e] = 0;
+                  for (int e = 0; e < 32; ++e) o[e] = 0;
                 }
 #pragma unroll
-                for (int y = 0; y < 2; ++y) {
+                for (int y = 0; y < 4; ++y) {
                   uint4 v;
                   v.x = ctx_pack2<FP16>(__uint_as_float(o[y * 8 + 0]) * inv, __uint_as_float(o[y * 8 + 1]) * inv);
                   v.y = ctx_pack2<FP16>(__uint_as_float(o[y * 8 + 2]) * inv, __uint_as_float(o[y * 8 + 3]) * inv);
                   v.z = ctx_pack2<FP16>(__uint_as_float(o[y * 8 + 4]) * inv, __uint_as_float(o[y * 8 + 5]) * inv);
                   v.w = ctx_pack2<FP16>(__uint_as_float(o[y * 8 + 6]) * inv, __uint_as_float(o[y * 8 + 7]) * inv);
-                  *reinterpret_cast<uint4*>(buf + (((c * 2 + y) ^ (lane & 7)) << 4)) = v;  // 128B swizzle
+                  *reinterpret_cast<uint4*>(buf + lane * 128 + (((c * 4 + y) ^ (lane & 7)) << 4)) = v;  // 128B swizzle
                 }
               }
               fence_proxy_async_smem();
               __syncwarp();
-              if (lane == 0 && first_tok < p.c.Sq) {
-                tma_store_4d(&tmO, stage + x * 4096, x * 64, t.hg * p.pack, first_tok, t.b);
+              if (lane == 0) {
+                if (first_tok < p.c.Sq) tma_store_4d(&tmO, buf, x * 64, t.hg * p.pack, first_tok, t.b);
                 tma_store_commit();
               }
             }
@@ -579,23 +619,24 @@ __global__ void __launch_bounds__(512, 1)
     } else if (warp == 3) {
       // ------------------------------ item decoder ------------------------------
       int4* ring = reinterpret_cast<int4*>(smem + CT_ITEM_OFF);
-      if (lane == 0) {
-        int n = 0;
-        for (int i = blockIdx.x;; i += gridDim.x, ++n) {
-          const bool end = i >= p.n_items;
-          if (!end)
-            t = ctx_item(p, i);
-          else
-            t.b = -1, t.hg = t.qp = t.split = t.first = t.len = t.j0 = t.nb = 0;
-          const int slot = n % CT_ITEMS;
-          if (!mbar_wait(&i_empty[slot], ((n / CT_ITEMS) & 1) ^ 1, ctx, 54)) break;
+      int n = 0, ends_b = -1;
+      int2 ends = make_int2(0, 0);
+      for (int i = blockIdx.x;; i += gridDim.x, ++n) {
+        const bool end = i >= p.n_items;
+        if (!end)
+          t = ctx_item<MASK>(p, i, ends_b, ends);
+        else
+          t.b = -1, t.hg = t.qp = t.split = t.first = t.len = t.j0 = t.nb = 0;
+        const int slot = n % CT_ITEMS;
+        if (!mbar_wait_warp(&i_empty[slot], ((n / CT_ITEMS) & 1) ^ 1, ctx, 54)) break;
+        if (lane == 0) {
           ring[slot * 2] = make_int4(t.b, t.hg, t.qp, t.split);
           ring[slot * 2 + 1] = make_int4(t.first, t.len, t.j0, t.nb);
           mbar_arrive(&i_full[slot]);
-          if (end) break;
         }
+        if (end) break;
+        __syncwarp();
       }
-      __syncwarp();
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
@@ -654,17 +695,6 @@ static int ctx_pack(int G) { return (G & (G - 1)) == 0 && G <= 32 ? G : 1; }
 long ctx_tc_items(int B, int Sq, int H, int Hkv) {
   const int pack = ctx_pack(H / Hkv), tok = 128 / pack;
   return static_cast<long>(B) * (H / pack) * ((Sq + 2 * tok - 1) / (2 * tok));
-}
-
-// [batch][token][head][channel] tensor map; a dimension of one entry may have any stride (TMA wants multiples of 16).
-static int ctx_tmap(CUtensorMap* m, const void* base, int fp16, int D, int heads, long hs, long rows, long ss, int B, long bs,
-                    uint32_t box_c, uint32_t box_h, uint32_t box_s, int swizzle) {
-  uint64_t dims[4] = {static_cast<uint64_t>(D), static_cast<uint64_t>(heads), static_cast<uint64_t>(rows),
-                      static_cast<uint64_t>(B)};
-  uint64_t str[3] = {static_cast<uint64_t>(heads > 1 ? hs : 8) * 2, static_cast<uint64_t>(rows > 1 ? ss : 8) * 2,
-                     static_cast<uint64_t>(B > 1 ? bs : 8) * 2};
-  uint32_t box[4] = {box_c, box_h, box_s, 1};
-  return make_tmap(m, base, fp16 ? TM_F16 : TM_BF16, 4, dims, str, box, swizzle);
 }
 
 template <bool FP16, int DK, bool MASK>
