@@ -229,18 +229,23 @@ __device__ __forceinline__ void ctx_softmax_part(uint32_t tmem_s, uint32_t tmem_
     const int left = keys - c * 32;
     const uint32_t vis = (MASK ? words[c] : 0xffffffffu) & (left >= 32 ? 0xffffffffu : (1u << left) - 1u);
     tmem_ld_wait();
+    if (vis != 0xffffffffu) {
 #pragma unroll
-    for (int e = 0; e < 32; ++e)
-      if (!((vis >> e) & 1)) s[e] = 0xff800000u;  // -inf
+      for (int e = 0; e < 32; ++e)
+        if (!((vis >> e) & 1)) s[e] = 0xff800000u;  // -inf
+    }
   };
-  float mx = -INFINITY;
+  float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll 1
   for (int c = 0; c < chunks; ++c) {
     load(c);
 #pragma unroll
-    for (int e = 0; e < 32; e += 2) mx = fmax3(mx, __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+    for (int e = 0; e < 32; e += 4) {
+      mx0 = fmax3(mx0, __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+      mx1 = fmax3(mx1, __uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
+    }
   }
-  ctx_new_max<DK>(tmem_o, fmaxf(m_used, mx * scale_log2), first, m_used, l);
+  ctx_new_max<DK>(tmem_o, fmaxf(m_used, fmaxf(mx0, mx1) * scale_log2), first, m_used, l);
   const float neg = m_used == -INFINITY ? 0.f : -m_used;
   uint64_t ps[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll 1
@@ -336,14 +341,19 @@ __global__ void __launch_bounds__(512, 1)
         const int tile_tok = (t.qp * 2 + st) * p.tok;
         const int tok = tile_tok + row_tok, head = t.hg * p.pack + row_head;
         const bool row_ok = tok < p.c.Sq;
-        const long token = static_cast<long>(t.b) * p.c.Sq + tok;
         float2 m_l = make_float2(-INFINITY, 0.f);
         if (t.nb > 0) {
           if (!(ok = mbar_wait_warp(&l_full[st], (o_phase >> st) & 1, ctx, 56))) break;
           m_l = ml[st * 128 + row];
         }
         const float inv = m_l.y > 0.f ? 1.f / m_l.y : 0.f;
-        const float lse2 = m_l.y > 0.f ? m_l.x + log2f(m_l.y) : -INFINITY;
+        if (row_ok && (p.c.part_o || p.c.lse)) {
+          const float lse2 = m_l.y > 0.f ? m_l.x + log2f(m_l.y) : -INFINITY;
+          if (p.c.part_o)
+            p.c.part_lse[((static_cast<long>(p.c.slot0 + t.split) * p.c.B + t.b) * p.c.Sq + tok) * p.c.H + head] = lse2;
+          else
+            p.c.lse[(static_cast<long>(t.b) * p.c.H + head) * p.c.Sq + tok] = lse2 * 0.6931471805599453f;
+        }
         if (t.nb > 0) {
           if (!(ok = mbar_wait_warp(&o_final[st], (o_phase >> st) & 1, ctx, 57))) break;
           o_phase ^= 1u << st;
@@ -351,8 +361,7 @@ __global__ void __launch_bounds__(512, 1)
         }
         const uint32_t tmem_o = tmem_base + lane_addr + 256 + st * 128;
         if (p.c.part_o) {
-          const long at = (static_cast<long>(p.c.slot0 + t.split) * p.c.B * p.c.Sq + token) * p.c.H + head;
-          if (row_ok) p.c.part_lse[at] = lse2;
+          const long at = ((static_cast<long>(p.c.slot0 + t.split) * p.c.B + t.b) * p.c.Sq + tok) * p.c.H + head;
           if (t.nb > 0) {
             for (int c = 0; c < DK / 16; ++c) {
               uint32_t o[16];
@@ -367,9 +376,8 @@ __global__ void __launch_bounds__(512, 1)
             }
           }
         } else {
-          if (p.c.lse && row_ok)
-            p.c.lse[(static_cast<long>(t.b) * p.c.H + head) * p.c.Sq + tok] = lse2 * 0.6931471805599453f;
           const int first_tok = tile_tok + wq * 32 / p.pack;
+          const uint64_t inv2 = f2_pack(inv, inv);
 #pragma unroll
           for (int x = 0; x < NBOX; ++x) {
             if (x * 64 < p.c.D) {
@@ -389,10 +397,12 @@ __global__ void __launch_bounds__(512, 1)
 #pragma unroll
                 for (int y = 0; y < 4; ++y) {
                   uint4 v;
-                  v.x = ctx_pack2<FP16>(__uint_as_float(o[y * 8 + 0]) * inv, __uint_as_float(o[y * 8 + 1]) * inv);
-                  v.y = ctx_pack2<FP16>(__uint_as_float(o[y * 8 + 2]) * inv, __uint_as_float(o[y * 8 + 3]) * inv);
-                  v.z = ctx_pack2<FP16>(__uint_as_float(o[y * 8 + 4]) * inv, __uint_as_float(o[y * 8 + 5]) * inv);
-                  v.w = ctx_pack2<FP16>(__uint_as_float(o[y * 8 + 6]) * inv, __uint_as_float(o[y * 8 + 7]) * inv);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    float a, b;
+                    f2_unpack(f2_mul(f2_pack(__uint_as_float(o[y * 8 + e * 2]), __uint_as_float(o[y * 8 + e * 2 + 1])), inv2), a, b);
+                    (&v.x)[e] = ctx_pack2<FP16>(a, b);
+                  }
                   *reinterpret_cast<uint4*>(buf + lane * 128 + (((c * 4 + y) ^ (lane & 7)) << 4)) = v;  // 128B swizzle
                 }
               }
