@@ -1,7 +1,8 @@
 // Shared declarations of the context attention kernels: attention of query tokens to states of another length
 // (an encoder's text / audio / image states, a cached clip), with per-sample lengths, packed samples, key masks and
 // grouped heads. context_attn_tc.cu has the tensor-memory kernel for full query tiles, context_attn_rows.cu the kernel
-// for a few query rows and the join of partial results, context_attn_host.cu picks between them.
+// for a few query rows and the join of partial results, context_attn_short.cu the one for very short states;
+// context_attn_host.cu picks between them.
 #pragma once
 #include "tfb_api.h"
 #include "tfb_common.cuh"
@@ -58,6 +59,9 @@ inline int ctx_tmap(CUtensorMap* m, const void* base, int fp16, int D, int heads
 // Few query rows (Sq * H / Hkv <= CTX_FEW_ROWS) of every sample against its own keys.
 constexpr int CTX_FEW_ROWS = 32;
 int launch_ctx_rows(const CtxParams& p, int fp16, cudaStream_t st);
+// Many query rows against at most CTX_SHORT_KEYS rows of k / v (p.Skv, packed samples together); writes final results only.
+constexpr int CTX_SHORT_KEYS = 64;
+int launch_ctx_short(const CtxParams& p, int fp16, cudaStream_t st);
 // Joins p.ns slots of part_o / part_lse (slot0 = 0) into out and lse.
 int launch_ctx_join(const CtxParams& p, int fp16, cudaStream_t st);
 // Full query tiles. kp / vp: the shared prefix (p.P rows, strides in elements), visited before the sample's own keys.

@@ -1,7 +1,7 @@
 // C entry points of context attention: argument checks, the choice of kernels and key splits.
 //
-// Rows kernel (context_attn_rows.cu) when a sample has at most 32 query rows per key head, tensor-memory kernel
-// (context_attn_tc.cu) otherwise. A shared prefix is visited by the tensor-memory kernel as the first key blocks of every
+// Rows kernel (context_attn_rows.cu) when a sample has at most 32 query rows per key head; otherwise the short-state kernel
+// (context_attn_short.cu) up to 64 key rows in all and the tensor-memory kernel (context_attn_tc.cu) beyond. A shared prefix is visited by the tensor-memory kernel as the first key blocks of every
 // sample when the sample fills a query tile; below that the prefix is computed once for all samples - their tokens form
 // one batch entry - as slots of its own, the samples' own keys as further slots, and the join adds them up.
 #include "context_attn.cuh"
@@ -16,6 +16,7 @@ struct CtxPlan {
   bool apart;          // prefix in slots of its own
   int ns_prefix, ns;   // key splits of the prefix pass and of the (only or own-keys) pass
   bool rows_prefix, rows_own;
+  bool short_own;      // at most 64 key rows in all and no prefix: context_attn_short.cu
   int slots() const { return (apart ? ns_prefix : 0) + ns; }
 };
 
@@ -49,9 +50,10 @@ CtxPlan make_plan(const tfb_context_attn_args* a) {
   pl.rows_own = few_rows(a->Sq, a->H, a->Hkv) && (a->P == 0 || pl.apart);
   const long tokens = static_cast<long>(a->B) * a->Sq;
   pl.rows_prefix = few_rows(tokens, a->H, a->Hkv);
+  pl.short_own = !pl.rows_own && a->P == 0 && a->Skv <= CTX_SHORT_KEYS;
   // Packed samples: the longest may hold every row.
   const long keys = a->Skv + (pl.apart ? 0 : a->P);
-  pl.ns = pick_splits(pl.rows_own, a->B, a->Sq, a->H, a->Hkv, keys);
+  pl.ns = pl.short_own ? 1 : pick_splits(pl.rows_own, a->B, a->Sq, a->H, a->Hkv, keys);
   pl.ns_prefix = pl.apart ? pick_splits(pl.rows_prefix, 1, tokens, a->H, a->Hkv, a->P) : 0;
   return pl;
 }
@@ -122,9 +124,9 @@ extern "C" int tfb_context_attn(const tfb_context_attn_args* a, void* stream) {
                                : launch_ctx_tc(f, nullptr, 0, 0, nullptr, 0, 0, a->fp16, st))
       return e;
   }
-  if (int e = pl.rows_own
-                  ? launch_ctx_rows(p, a->fp16, st)
-                  : launch_ctx_tc(p, a->kp, a->kp_ss, a->kp_hs, a->vp, a->vp_ss, a->vp_hs, a->fp16, st))
+  if (int e = pl.rows_own ? launch_ctx_rows(p, a->fp16, st)
+              : pl.short_own ? launch_ctx_short(p, a->fp16, st)
+                             : launch_ctx_tc(p, a->kp, a->kp_ss, a->kp_hs, a->vp, a->vp_ss, a->vp_hs, a->fp16, st))
     return e;
   if (pl.slots() > 1) {
     p.ns = pl.slots();

@@ -163,11 +163,15 @@ TILES = [  # query tiles: one tile, two, odd numbers, grouped heads that share a
     (1, 17, 1, 1, 128, 1), (2, 128, 2, 2, 128, 128), (2, 129, 2, 1, 64, 257), (3, 300, 3, 1, 128, 77), (1, 64, 8, 1, 128, 515),
     (2, 257, 4, 4, 96, 512), (2, 31, 32, 1, 64, 33), (1, 1000, 2, 2, 40, 640), (4, 20, 6, 2, 128, 1100), (1, 130, 1, 1, 128, 9000),
 ]
+SHORT = [  # many query rows, at most 64 keys
+    (2, 40, 1, 1, 128, 1), (3, 1000, 3, 1, 64, 32), (2, 333, 4, 2, 128, 64), (2, 100, 10, 2, 72, 17), (1, 5000, 2, 2, 40, 63),
+    (9, 65, 16, 4, 128, 50),
+]
 
 
 @gpu
 @pytest.mark.parametrize("dtype", [BF, FP])
-@pytest.mark.parametrize("shape", ROWS + TILES)
+@pytest.mark.parametrize("shape", ROWS + TILES + SHORT)
 def test_dense(lib, shape, dtype):
     q, k, v = make(*shape, dtype, "cuda")
     o, lse = CA.cross_attention(q, k, v, return_lse=True)
@@ -175,7 +179,7 @@ def test_dense(lib, shape, dtype):
 
 
 @gpu
-@pytest.mark.parametrize("shape", ROWS + TILES)
+@pytest.mark.parametrize("shape", ROWS + TILES + SHORT)
 @pytest.mark.parametrize("layout", ["padded", "packed", "masked", "masked_lens"])
 def test_lengths_and_masks(lib, shape, layout):
     """Ragged samples, one of them empty; what is hidden holds NaN and infinities."""
