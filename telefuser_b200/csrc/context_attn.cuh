@@ -11,8 +11,9 @@
 namespace tfb {
 
 struct CtxParams {
-  const void *q, *k, *v;
+  const void *q, *k, *v, *kp, *vp;
   long q_bs, q_ss, q_hs, k_bs, k_ss, k_hs, v_bs, v_ss, v_hs;  // element strides of batch, token, head
+  long kp_ss, kp_hs, vp_ss, vp_hs;                             // the shared prefix has one batch entry
   void* out;        // [B, Sq, H, D] contiguous
   float* lse;       // [B, H, Sq] or null
   float* part_o;    // non-null: results go to slots [slot][B * Sq][H][D] (each slot normalised by its own sum) ...
@@ -56,7 +57,7 @@ inline int ctx_tmap(CUtensorMap* m, const void* base, int fp16, int D, int heads
   return make_tmap(m, base, fp16 ? TM_F16 : TM_BF16, 4, dims, str, box, swizzle);
 }
 
-// Few query rows (Sq * H / Hkv <= CTX_FEW_ROWS) of every sample against its own keys.
+// Few query rows (Sq * H / Hkv <= CTX_FEW_ROWS) of every sample against the prefix and its own keys.
 constexpr int CTX_FEW_ROWS = 32;
 int launch_ctx_rows(const CtxParams& p, int fp16, cudaStream_t st);
 // Many query rows against at most CTX_SHORT_KEYS rows of k / v (p.Skv, packed samples together); writes final results only.
@@ -64,9 +65,8 @@ constexpr int CTX_SHORT_KEYS = 64;
 int launch_ctx_short(const CtxParams& p, int fp16, cudaStream_t st);
 // Joins p.ns slots of part_o / part_lse (slot0 = 0) into out and lse.
 int launch_ctx_join(const CtxParams& p, int fp16, cudaStream_t st);
-// Full query tiles. kp / vp: the shared prefix (p.P rows, strides in elements), visited before the sample's own keys.
-int launch_ctx_tc(const CtxParams& p, const void* kp, long kp_ss, long kp_hs, const void* vp, long vp_ss, long vp_hs,
-                  int fp16, cudaStream_t st);
+// Full query tiles against the prefix and the sample's own keys.
+int launch_ctx_tc(const CtxParams& p, int fp16, cudaStream_t st);
 // Work items of launch_ctx_tc with p.ns = 1.
 long ctx_tc_items(int B, int Sq, int H, int Hkv);
 

@@ -1,9 +1,11 @@
 // C entry points of context attention: argument checks, the choice of kernels and key splits.
 //
 // Rows kernel (context_attn_rows.cu) when a sample has at most 32 query rows per key head; otherwise the short-state kernel
-// (context_attn_short.cu) up to 64 key rows in all and the tensor-memory kernel (context_attn_tc.cu) beyond. A shared prefix is visited by the tensor-memory kernel as the first key blocks of every
-// sample when the sample fills a query tile; below that the prefix is computed once for all samples - their tokens form
-// one batch entry - as slots of its own, the samples' own keys as further slots, and the join adds them up.
+// (context_attn_short.cu) up to 64 key rows in all and the tensor-memory kernel (context_attn_tc.cu) beyond.
+// A shared prefix is visited as the first keys of every sample while re-reading it costs little: always when a sample fills a
+// query tile, and below that while the batch's re-reads stay small enough for L2. Otherwise it is computed once for all
+// samples - their tokens form one batch entry - as slots of its own, the samples' own keys as further slots, and the join
+// adds them up: two more launches, which 16 MB of re-reads cost about as much as.
 #include "context_attn.cuh"
 
 using namespace tfb;
@@ -11,6 +13,7 @@ using namespace tfb;
 namespace {
 
 constexpr int CTX_MAX_SPLITS = 64;
+constexpr long CTX_REREAD_BYTES = 16 << 20;
 
 struct CtxPlan {
   bool apart;          // prefix in slots of its own
@@ -23,12 +26,13 @@ struct CtxPlan {
 bool few_rows(long tokens, int H, int Hkv) { return tokens * (H / Hkv) <= CTX_FEW_ROWS; }
 
 // Splits of the key range so that few items still fill the device: two CTAs per SM for the rows kernel (two are
-// resident), one per SM for the tensor-memory kernel; a slice is never shorter than what a CTA takes in one step.
+// resident), one per SM for the tensor-memory kernel. A slice has no fewer than 512 and 256 keys: below that the join and
+// its launch cost more than the slice saves (one token of 8 streams against 512 keys: 8.0 us in two slices and a join).
 int pick_splits(bool rows, int B, long Sq, int H, int Hkv, long keys) {
   const long sms = sm_count();
   const long items = rows ? static_cast<long>(B) * Hkv : ctx_tc_items(B, static_cast<int>(Sq), H, Hkv);
   long ns = (rows ? 2 * sms : sms) / (items > 0 ? items : 1);
-  const long most = (keys + 127) / 128 / (rows ? 1 : 2);
+  const long most = keys / (rows ? 512 : 256);
   if (ns > most) ns = most;
   if (ns > CTX_MAX_SPLITS) ns = CTX_MAX_SPLITS;
   return ns < 1 ? 1 : static_cast<int>(ns);
@@ -46,8 +50,9 @@ int check(const tfb_context_attn_args* a) {
 CtxPlan make_plan(const tfb_context_attn_args* a) {
   CtxPlan pl;
   const int G = a->H / a->Hkv;
-  pl.apart = a->P > 0 && static_cast<long>(a->Sq) * G < 128;
-  pl.rows_own = few_rows(a->Sq, a->H, a->Hkv) && (a->P == 0 || pl.apart);
+  const long reread = 4L * a->P * a->Hkv * a->D * (a->B - 1);  // bytes of K and V
+  pl.apart = a->P > 0 && a->B > 1 && static_cast<long>(a->Sq) * G < 128 && reread > CTX_REREAD_BYTES;
+  pl.rows_own = few_rows(a->Sq, a->H, a->Hkv);
   const long tokens = static_cast<long>(a->B) * a->Sq;
   pl.rows_prefix = few_rows(tokens, a->H, a->Hkv);
   pl.short_own = !pl.rows_own && a->P == 0 && a->Skv <= CTX_SHORT_KEYS;
@@ -86,6 +91,8 @@ extern "C" int tfb_context_attn(const tfb_context_attn_args* a, void* stream) {
   p.q_bs = a->q_bs, p.q_ss = a->q_ss, p.q_hs = a->q_hs;
   p.k_bs = a->k_bs, p.k_ss = a->k_ss, p.k_hs = a->k_hs;
   p.v_bs = a->v_bs, p.v_ss = a->v_ss, p.v_hs = a->v_hs;
+  p.kp = a->kp, p.vp = a->vp;
+  p.kp_ss = a->kp_ss, p.kp_hs = a->kp_hs, p.vp_ss = a->vp_ss, p.vp_hs = a->vp_hs;
   p.out = a->out;
   p.lse = a->lse;
   p.kv_lens = a->kv_lens;
@@ -120,13 +127,11 @@ extern "C" int tfb_context_attn(const tfb_context_attn_args* a, void* stream) {
     f.B = 1, f.Sq = static_cast<int>(tokens), f.Skv = a->P;
     f.ns = pl.ns_prefix;
     f.slot0 = 0;
-    if (int e = pl.rows_prefix ? launch_ctx_rows(f, a->fp16, st)
-                               : launch_ctx_tc(f, nullptr, 0, 0, nullptr, 0, 0, a->fp16, st))
-      return e;
+    if (int e = pl.rows_prefix ? launch_ctx_rows(f, a->fp16, st) : launch_ctx_tc(f, a->fp16, st)) return e;
   }
   if (int e = pl.rows_own ? launch_ctx_rows(p, a->fp16, st)
               : pl.short_own ? launch_ctx_short(p, a->fp16, st)
-                             : launch_ctx_tc(p, a->kp, a->kp_ss, a->kp_hs, a->vp, a->vp_ss, a->vp_hs, a->fp16, st))
+                             : launch_ctx_tc(p, a->fp16, st))
     return e;
   if (pl.slots() > 1) {
     p.ns = pl.slots();

@@ -21,7 +21,8 @@ constexpr int CR_WARPS = 4;
 
 struct CtxRowsParams {
   CtxParams c;
-  int bmul;  // 0: packed samples, the tensors have one batch entry
+  int bmul;      // 0: packed samples, the tensors have one batch entry
+  int n_prefix;  // 16-key chunks of the shared prefix, in front of the sample's own
 };
 
 template <bool FP16>
@@ -68,6 +69,7 @@ struct CtxRowsCfg {
 template <bool FP16, int DK, int MT>
 __global__ void __launch_bounds__(CR_WARPS * 32, 2)
     ctx_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                    const __grid_constant__ CUtensorMap tmKp, const __grid_constant__ CUtensorMap tmVp,
                     const __grid_constant__ CtxRowsParams rp) {
   using Cfg = CtxRowsCfg<DK, MT>;
   constexpr int NBOX = DK / 64, ROWS = MT * 16;
@@ -85,7 +87,7 @@ __global__ void __launch_bounds__(CR_WARPS * 32, 2)
   const int b = blockIdx.x / p.ns / p.Hkv;
   int first, len;
   ctx_sample_range(p, b, first, len);
-  const long n16 = (len + 15) >> 4;
+  const long n16 = rp.n_prefix + ((len + 15) >> 4);
   const int i0 = static_cast<int>(n16 * split / p.ns), i1 = static_cast<int>(n16 * (split + 1) / p.ns);
 
   uint64_t* full = bars + warp * Cfg::STAGES;
@@ -94,10 +96,12 @@ __global__ void __launch_bounds__(CR_WARPS * 32, 2)
   auto fetch = [&](int it, int slot) {
     uint8_t* dst = ring + slot * Cfg::CHUNK;
     mbar_expect_tx(&full[slot], Cfg::CHUNK);
+    const bool pre = it < rp.n_prefix;
+    const int row = pre ? it * 16 : first + (it - rp.n_prefix) * 16, bb = pre ? 0 : b * rp.bmul;
 #pragma unroll
     for (int x = 0; x < NBOX; ++x) {
-      tma_load_4d(dst + x * 2048, &tmK, &full[slot], x * 64, hk, first + it * 16, b * rp.bmul);
-      tma_load_4d(dst + (NBOX + x) * 2048, &tmV, &full[slot], x * 64, hk, first + it * 16, b * rp.bmul);
+      tma_load_4d(dst + x * 2048, pre ? &tmKp : &tmK, &full[slot], x * 64, hk, row, bb);
+      tma_load_4d(dst + (NBOX + x) * 2048, pre ? &tmVp : &tmV, &full[slot], x * 64, hk, row, bb);
     }
   };
   if (lane == 0) {
@@ -140,11 +144,13 @@ __global__ void __launch_bounds__(CR_WARPS * 32, 2)
   uint32_t phase = 0;
   for (int it = i0 + warp; it < i1; it += CR_WARPS) {
     // keys of this lane's score columns: 2c, 2c + 1, 2c + 8, 2c + 9 of the chunk
+    const bool pre = it < rp.n_prefix;
+    const int keys = pre ? p.P : len;
     bool vis[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int j = it * 16 + 2 * c + (e & 1) + (e >> 1) * 8;
-      vis[e] = j < len && (!mb || mb[j]);
+      const int j = (pre ? it : it - rp.n_prefix) * 16 + 2 * c + (e & 1) + (e >> 1) * 8;
+      vis[e] = j < keys && (!mb || mb[j]);
     }
     // after an expired wait (recorded in the status word) the warp goes on with what is there, to the common end
     mbar_wait_warp(&full[slot], phase, ctx, 80);
@@ -332,17 +338,21 @@ static int launch_ctx_rows_impl(const CtxParams& p, cudaStream_t st) {
   CtxRowsParams rp;
   rp.c = p;
   rp.bmul = p.cu_kv ? 0 : 1;
-  CUtensorMap tk, tv;
+  rp.n_prefix = (p.P + 15) / 16;
+  CUtensorMap tk, tv, tkp, tvp;
+  memset(&tk, 0, sizeof(tk));  // a map without rows is not used
+  tv = tkp = tvp = tk;
+  int e;
   if (p.Skv > 0) {
     const int kb = p.cu_kv ? 1 : p.B;
-    int e;
     if ((e = ctx_tmap(&tk, p.k, FP16, p.D, p.Hkv, p.k_hs, p.Skv, p.k_ss, kb, p.k_bs, 64, 1, 16, TM_SW_128))) return e;
     if ((e = ctx_tmap(&tv, p.v, FP16, p.D, p.Hkv, p.v_hs, p.Skv, p.v_ss, kb, p.v_bs, 64, 1, 16, TM_SW_128))) return e;
-  } else {  // no keys at all: the maps are not used
-    memset(&tk, 0, sizeof(tk));
-    memset(&tv, 0, sizeof(tv));
   }
-  kern<<<static_cast<int>(ctas), CR_WARPS * 32, Cfg::SMEM, st>>>(tk, tv, rp);
+  if (p.P > 0) {
+    if ((e = ctx_tmap(&tkp, p.kp, FP16, p.D, p.Hkv, p.kp_hs, p.P, p.kp_ss, 1, 0, 64, 1, 16, TM_SW_128))) return e;
+    if ((e = ctx_tmap(&tvp, p.vp, FP16, p.D, p.Hkv, p.vp_hs, p.P, p.vp_ss, 1, 0, 64, 1, 16, TM_SW_128))) return e;
+  }
+  kern<<<static_cast<int>(ctas), CR_WARPS * 32, Cfg::SMEM, st>>>(tk, tv, tkp, tvp, rp);
   return cudaGetLastError() == cudaSuccess ? TFB_OK : TFB_ERR_LAUNCH;
 }
 

@@ -1,24 +1,25 @@
 // Context attention of many query rows to at most 64 keys (audio windows, image tokens, short prompts): HBM bound on the
 // queries and the output, 1 KB per row and head dim 128 against a few thousand tensor operations.
 //
-// So nothing stands between memory and registers but warps: a CTA of eight keeps the keys and values of one (sample, key
+// So nothing stands between memory and registers but warps: a CTA of four keeps the keys and values of one (sample, key
 // head) in shared memory, and every warp takes tiles of 16 query rows - (token, grouped head) pairs, any group size - straight
 // from global memory into mma.sync fragments, softmax in registers, results straight to global memory, the next tile's
-// queries already on their way. 16 warps per SM hold about 64 KB of loads in flight. (The tensor-memory kernel hands every
+// queries already on their way. 16 to 20 warps per SM hold 64 KB and more of loads in flight. (The tensor-memory kernel hands every
 // tile through five warps and their barriers, which costs it about 10,000 clk per 256 rows whatever the keys: 258 us against
 // this kernel's figure for 21 frames of 1560 tokens x 40 heads against 32 keys.)
 // Coalescing comes from permuting indexes: a lane loads and stores whole 16-byte pieces of a row, and the copies of K and V
 // in shared memory have their channels reordered to match what the fragments then hold:
 //   Q.K^T  lane (n, c) = (lane / 4, lane % 4) holds channels 32 i + 8 c .. + 7 of row n, i.e. of k-step u = 0, 1 the pairs
 //          4 u + 2 h (h = 0, 1): K stores channel 32 i + 8 c + 4 u + 2 h + e at position 32 i + 16 u + 8 h + 2 c + e
-//   P.V    column 2 c + e of tile t is channel 64 blk + 16 c + 8 e + t: V stores channel 64 blk + 8 n + t at 64 blk + 8 t + n
+//   P.V    column 2 c + e of tile t is channel 64 blk + 32 e + 8 c + t, so that the four lanes of a row store 64 bytes next to
+//          each other: V stores that channel at position 64 blk + 8 t + 2 c + e
 // Hidden keys are zeros in both copies and their scores become -inf, so what lies there does not matter.
 #include "context_attn.cuh"
 
 namespace tfb {
 
-constexpr int CS_WARPS = 8;
-constexpr int CS_KEYS = CTX_SHORT_KEYS;
+constexpr int CS_WARPS = 4;
+static_assert(CTX_SHORT_KEYS == 64, "four steps of 16 keys");
 
 struct CtxShortParams {
   CtxParams c;
@@ -40,19 +41,21 @@ __device__ __forceinline__ void cs_mma(float (&d)[4], uint32_t a0, uint32_t a1, 
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <bool FP16, int DK>
-__global__ void __launch_bounds__(CS_WARPS * 32, 2) ctx_short_kernel(const __grid_constant__ CtxShortParams sp) {
+// STEPS: 16-key steps that the registers are laid out for (2 or 4).
+template <bool FP16, int DK, int STEPS>
+__global__ void __launch_bounds__(CS_WARPS * 32, STEPS == 2 ? 5 : 4) ctx_short_kernel(const __grid_constant__ CtxShortParams sp) {
   constexpr int NCH = DK / 32, NBLK = DK / 64, LD = DK + 8;  // row stride: 16 bytes over a multiple of 128
-  __shared__ __align__(16) uint16_t s_k[CS_KEYS * LD];
-  __shared__ __align__(16) uint16_t s_v[CS_KEYS * LD];
+  __shared__ __align__(16) uint16_t s_k[STEPS * 16 * LD];
+  __shared__ __align__(16) uint16_t s_v[STEPS * 16 * LD];
   const CtxParams& p = sp.c;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n = lane >> 2, c = lane & 3;
   const int G = p.H / p.Hkv;
   const unsigned uG = G, R = static_cast<unsigned>(p.Sq) * uG;  // below 2^31
-  const int chunk = blockIdx.x % sp.chunks;
-  const int hk = (blockIdx.x / sp.chunks) % p.Hkv;
-  const int b = blockIdx.x / sp.chunks / p.Hkv;
+  // Heads first: CTAs that run at the same time then read and write the heads of the same tokens, whole DRAM pages together.
+  const int hk = blockIdx.x % p.Hkv;
+  const int chunk = (blockIdx.x / p.Hkv) % sp.chunks;
+  const int b = blockIdx.x / p.Hkv / sp.chunks;
   const int t0 = chunk * sp.per_cta, t1 = min(t0 + sp.per_cta, sp.tiles);
 
   const uint16_t* qb = static_cast<const uint16_t*>(p.q) + static_cast<long>(b) * p.q_bs + static_cast<long>(hk) * G * p.q_hs;
@@ -74,7 +77,7 @@ __global__ void __launch_bounds__(CS_WARPS * 32, 2) ctx_short_kernel(const __gri
 
   int first, len;
   ctx_sample_range(p, b, first, len);
-  len = min(len, CS_KEYS);  // packed samples: the rule on sizes has looked at all their rows
+  len = min(len, STEPS * 16);  // packed samples: the rule on sizes has looked at all their rows
   const uint8_t* mb = p.key_mask ? p.key_mask + static_cast<long>(b) * p.mask_bs : nullptr;
   const int steps = (len + 15) >> 4;  // 16 keys each
   const long kv_b = p.cu_kv ? 0 : b;
@@ -89,7 +92,7 @@ __global__ void __launch_bounds__(CS_WARPS * 32, 2) ctx_short_kernel(const __gri
       vw = __ldg(reinterpret_cast<const uint4*>(vb + static_cast<long>(key) * p.v_ss + ch));
     }
     uint16_t* kd = s_k + key * LD + (ch & ~31) + (ch >> 3 & 3) * 2;
-    uint16_t* vd = s_v + key * LD + (ch & ~63) + (ch >> 3 & 7);
+    uint16_t* vd = s_v + key * LD + (ch & ~63) + (ch >> 3 & 3) * 2 + (ch >> 5 & 1);
 #pragma unroll
     for (int w = 0; w < 4; ++w) {  // word w: channels ch + 2 w, + 1; u = w / 2, h = w % 2
       *reinterpret_cast<uint32_t*>(kd + (w >> 1) * 16 + (w & 1) * 8) = (&kw.x)[w];
@@ -100,10 +103,11 @@ __global__ void __launch_bounds__(CS_WARPS * 32, 2) ctx_short_kernel(const __gri
   // hidden keys among this lane's score columns 16 step + 8 t + 2 c + e, as bits 4 step + 2 t + e
   uint32_t hidden = 0;
 #pragma unroll
-  for (int x = 0; x < CS_KEYS / 4; ++x) {
+  for (int x = 0; x < STEPS * 4; ++x) {
     const int key = (x >> 2) * 16 + (x >> 1 & 1) * 8 + 2 * c + (x & 1);
     if (key >= len || (mb && !mb[key])) hidden |= 1u << x;
   }
+  const bool some_hidden = __any_sync(0xffffffffu, hidden != 0);
   __syncthreads();
 
   // ldmatrix rows of this lane (see context_attn_rows.cu): K by key octets, V by key rows of a 16-key step
@@ -112,9 +116,9 @@ __global__ void __launch_bounds__(CS_WARPS * 32, 2) ctx_short_kernel(const __gri
   uint16_t* ob = static_cast<uint16_t*>(p.out) + (static_cast<long>(b) * p.Sq * p.H + static_cast<long>(hk) * G) * p.D;
 
   for (int tile = t0 + warp; tile < t1; tile += CS_WARPS) {
-    float s[CS_KEYS / 16][2][4];
+    float s[STEPS][2][4];
 #pragma unroll
-    for (int st = 0; st < CS_KEYS / 16; ++st) {
+    for (int st = 0; st < STEPS; ++st) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -137,32 +141,35 @@ __global__ void __launch_bounds__(CS_WARPS * 32, 2) ctx_short_kernel(const __gri
     }
     load_q(tile + CS_WARPS);
     float inv[2], lse2[2];
-    uint32_t pf[CS_KEYS / 16][4];
+    uint32_t pf[STEPS][4];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
+      if (some_hidden) {
+#pragma unroll
+        for (int x = 0; x < STEPS * 4; ++x)
+          if (hidden >> x & 1) s[x >> 2][x >> 1 & 1][r * 2 + (x & 1)] = -INFINITY;
+      }
       float mx = -INFINITY;
 #pragma unroll
-      for (int x = 0; x < CS_KEYS / 4; ++x) {
-        float& v = s[x >> 2][x >> 1 & 1][r * 2 + (x & 1)];
-        v = hidden >> x & 1 ? -INFINITY : v * p.scale_log2;
-        mx = fmaxf(mx, v);
-      }
+      for (int st = 0; st < STEPS; ++st)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) mx = fmax3(mx, s[st][t][r * 2], s[st][t][r * 2 + 1]);
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float base = mx == -INFINITY ? 0.f : mx;
+      const float base = mx == -INFINITY ? 0.f : mx * p.scale_log2;
       float l = 0.f;
 #pragma unroll
-      for (int st = 0; st < CS_KEYS / 16; ++st)
+      for (int st = 0; st < STEPS; ++st)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const float p0 = fast_exp2(s[st][t][r * 2] - base), p1 = fast_exp2(s[st][t][r * 2 + 1] - base);
+          const float p0 = fast_exp2(s[st][t][r * 2] * p.scale_log2 - base), p1 = fast_exp2(s[st][t][r * 2 + 1] * p.scale_log2 - base);
           l += p0 + p1;
           pf[st][t * 2 + r] = ctx_pack2<FP16>(p0, p1);  // in [0, 1], rounded to the inputs' type for the product
         }
       l += __shfl_xor_sync(0xffffffffu, l, 1);
       l += __shfl_xor_sync(0xffffffffu, l, 2);
       inv[r] = l > 0.f ? 1.f / l : 0.f;
-      lse2[r] = l > 0.f ? mx + log2f(l) : -INFINITY;
+      lse2[r] = l > 0.f ? base + log2f(l) : -INFINITY;
     }
     long row_at[2];
     bool row_ok[2];
@@ -183,7 +190,7 @@ __global__ void __launch_bounds__(CS_WARPS * 32, 2) ctx_short_kernel(const __gri
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[t][e] = 0.f;
 #pragma unroll
-      for (int st = 0; st < CS_KEYS / 16; ++st) {
+      for (int st = 0; st < STEPS; ++st) {
         if (st < steps) {
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
@@ -200,7 +207,7 @@ __global__ void __launch_bounds__(CS_WARPS * 32, 2) ctx_short_kernel(const __gri
       for (int r = 0; r < 2; ++r)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int d = blk * 64 + 16 * c + 8 * e;
+          const int d = blk * 64 + 32 * e + 8 * c;
           uint4 w;
 #pragma unroll
           for (int x = 0; x < 4; ++x) (&w.x)[x] = ctx_pack2<FP16>(o[2 * x][r * 2 + e] * inv[r], o[2 * x + 1][r * 2 + e] * inv[r]);
@@ -210,7 +217,7 @@ __global__ void __launch_bounds__(CS_WARPS * 32, 2) ctx_short_kernel(const __gri
   }
 }
 
-template <bool FP16, int DK>
+template <bool FP16, int DK, int STEPS>
 static int launch_ctx_short_impl(const CtxParams& p, cudaStream_t st) {
   CtxShortParams sp;
   sp.c = p;
@@ -219,23 +226,29 @@ static int launch_ctx_short_impl(const CtxParams& p, cudaStream_t st) {
   if (rows > 0x7fffff00L) return TFB_ERR_TOO_LARGE;
   // About eight CTAs per resident one, so that the last wave is short, but no fewer than four tiles per warp: refilling
   // shared memory with K and V should stay small against them.
-  const long want = (8L * 2 * sm_count() + heads - 1) / heads;
+  const long want = (8L * 4 * sm_count() + heads - 1) / heads;
   long per = (tiles + want - 1) / want;
   if (per < 4 * CS_WARPS) per = 4 * CS_WARPS;
-  if (heads * ((tiles + per - 1) / per) < 2 * sm_count()) per = CS_WARPS;
+  if (heads * ((tiles + per - 1) / per) < 4 * sm_count()) per = CS_WARPS;
   sp.tiles = static_cast<int>(tiles);
   sp.per_cta = static_cast<int>((per + CS_WARPS - 1) / CS_WARPS * CS_WARPS);
   sp.chunks = static_cast<int>((tiles + sp.per_cta - 1) / sp.per_cta);
   const long ctas = heads * sp.chunks;
   if (ctas > 0x7fffffffL) return TFB_ERR_TOO_LARGE;
-  ctx_short_kernel<FP16, DK><<<static_cast<int>(ctas), CS_WARPS * 32, 0, st>>>(sp);
+  ctx_short_kernel<FP16, DK, STEPS><<<static_cast<int>(ctas), CS_WARPS * 32, 0, st>>>(sp);
   return cudaGetLastError() == cudaSuccess ? TFB_OK : TFB_ERR_LAUNCH;
+}
+
+template <bool FP16>
+static int launch_ctx_short_type(const CtxParams& p, cudaStream_t st) {
+  const bool two = p.Skv <= 32;
+  if (p.D <= 64) return two ? launch_ctx_short_impl<FP16, 64, 2>(p, st) : launch_ctx_short_impl<FP16, 64, 4>(p, st);
+  return two ? launch_ctx_short_impl<FP16, 128, 2>(p, st) : launch_ctx_short_impl<FP16, 128, 4>(p, st);
 }
 
 int launch_ctx_short(const CtxParams& p, int fp16, cudaStream_t st) {
   if (p.Skv > CTX_SHORT_KEYS || p.part_o) return TFB_ERR_TOO_LARGE;
-  if (p.D <= 64) return fp16 ? launch_ctx_short_impl<true, 64>(p, st) : launch_ctx_short_impl<false, 64>(p, st);
-  return fp16 ? launch_ctx_short_impl<true, 128>(p, st) : launch_ctx_short_impl<false, 128>(p, st);
+  return fp16 ? launch_ctx_short_type<true>(p, st) : launch_ctx_short_type<false>(p, st);
 }
 
 }  // namespace tfb

@@ -717,8 +717,7 @@ static int launch_ctx_tc_impl(const CUtensorMap (&tm)[6], const CtxTcParams& p, 
   return cudaGetLastError() == cudaSuccess ? TFB_OK : TFB_ERR_LAUNCH;
 }
 
-int launch_ctx_tc(const CtxParams& c, const void* kp, long kp_ss, long kp_hs, const void* vp, long vp_ss, long vp_hs,
-                  int fp16, cudaStream_t st) {
+int launch_ctx_tc(const CtxParams& c, int fp16, cudaStream_t st) {
   CtxTcParams p;
   p.c = c;
   p.pack = ctx_pack(c.H / c.Hkv);
@@ -740,8 +739,8 @@ int launch_ctx_tc(const CtxParams& c, const void* kp, long kp_ss, long kp_hs, co
     if ((e = ctx_tmap(&tm[2], c.v, fp16, c.D, c.Hkv, c.v_hs, c.Skv, c.v_ss, kb, c.v_bs, 64, 1, 128, TM_SW_128))) return e;
   }
   if (c.P > 0) {
-    if ((e = ctx_tmap(&tm[3], kp, fp16, c.D, c.Hkv, kp_hs, c.P, kp_ss, 1, 0, 64, 1, 128, TM_SW_128))) return e;
-    if ((e = ctx_tmap(&tm[4], vp, fp16, c.D, c.Hkv, vp_hs, c.P, vp_ss, 1, 0, 64, 1, 128, TM_SW_128))) return e;
+    if ((e = ctx_tmap(&tm[3], c.kp, fp16, c.D, c.Hkv, c.kp_hs, c.P, c.kp_ss, 1, 0, 64, 1, 128, TM_SW_128))) return e;
+    if ((e = ctx_tmap(&tm[4], c.vp, fp16, c.D, c.Hkv, c.vp_hs, c.P, c.vp_ss, 1, 0, 64, 1, 128, TM_SW_128))) return e;
   } else {
     tm[3] = c.Skv > 0 ? tm[1] : tm[0], tm[4] = c.Skv > 0 ? tm[2] : tm[0];
   }

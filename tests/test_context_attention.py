@@ -214,7 +214,7 @@ def test_lengths_and_masks(lib, shape, layout):
 @pytest.mark.parametrize("shape,P", [
     ((1, 1, 1, 1, 64, 1), 1), ((3, 4, 8, 2, 64, 33), 77), ((64, 1, 8, 2, 128, 100), 1000), ((5, 1, 4, 4, 128, 1), 3000),
     ((2, 7, 6, 2, 128, 65), 130), ((2, 300, 2, 2, 128, 129), 257), ((2, 128, 4, 1, 64, 200), 64), ((1, 500, 2, 1, 96, 77), 600),
-    ((3, 40, 2, 2, 128, 0), 100), ((3, 2, 2, 2, 128, 50), 0), ((2, 200, 2, 2, 128, 50), 0), ((2, 200, 2, 2, 128, 0), 50),
+    ((3, 40, 2, 2, 128, 0), 100), ((20, 2, 4, 2, 64, 70), 9000), ((9, 1, 24, 8, 128, 20), 2500), ((3, 2, 2, 2, 128, 50), 0), ((2, 200, 2, 2, 128, 50), 0), ((2, 200, 2, 2, 128, 0), 50),
 ])  # fmt: skip
 @pytest.mark.parametrize("ragged", [False, True])
 def test_prefix(lib, shape, P, ragged, dtype):
