@@ -35,7 +35,7 @@ constexpr int CT_OUT_OFF = CT_KV_OFF + 4 * CT_TILE;  // 4 output warps x 2 boxes
 constexpr int CT_ML_OFF = CT_OUT_OFF + 4 * 8192;     // [2 tiles][128 rows] of (maximum, sum)
 constexpr int CT_ITEMS = 4;                          // ring of decoded items
 constexpr int CT_ITEM_OFF = CT_ML_OFF + 2 * 128 * 8;
-constexpr int CT_BAR_OFF = CT_ITEM_OFF + CT_ITEMS * 32;
+constexpr int CT_BAR_OFF = CT_ITEM_OFF + CT_ITEMS * 48;
 constexpr int CT_N_BARS = 20 + 2 * CT_ITEMS;
 constexpr int CT_ALIGN_SLACK = 512;  // dynamic shared memory starts on 1 KB here; the kernel checks that the tiles fit
 constexpr int CT_SMEM_BYTES = CT_BAR_OFF + CT_N_BARS * 8 + 64 + CT_ALIGN_SLACK;
@@ -130,7 +130,7 @@ struct CtxItems {
     const int slot = n % CT_ITEMS;
     if (!mbar_wait_warp(&full[slot], (n / CT_ITEMS) & 1, ctx, site)) return false;
     ++n;
-    const int4 a = ring[slot * 2], b = ring[slot * 2 + 1];
+    const int4 a = ring[slot * 3], b = ring[slot * 3 + 1];
     __syncwarp();
     if (lane_id() == 0) mbar_arrive(&empty[slot]);
     t.b = __shfl_sync(0xffffffffu, a.x, 0), t.hg = __shfl_sync(0xffffffffu, a.y, 0);
@@ -138,6 +138,22 @@ struct CtxItems {
     t.first = __shfl_sync(0xffffffffu, b.x, 0), t.len = __shfl_sync(0xffffffffu, b.y, 0);
     t.j0 = __shfl_sync(0xffffffffu, b.z, 0), t.nb = __shfl_sync(0xffffffffu, b.w, 0);
     return t.b >= 0;
+  }
+  // What the issuer needs of the next item with keys: blocks, query tiles, the place of the prefix's last block among them
+  // (or -1), and the columns of that block (low half) and of the item's last. False as above.
+  __device__ __forceinline__ bool next_issue(int4& r, const AbortCtx& ctx, int site) {
+    do {
+      const int slot = n % CT_ITEMS;
+      if (!mbar_wait_warp(&full[slot], (n / CT_ITEMS) & 1, ctx, site)) return false;
+      ++n;
+      if (lane_id() == 0) {
+        r = ring[slot * 3 + 2];
+        mbar_arrive(&empty[slot]);
+      }
+      r.x = __shfl_sync(0xffffffffu, r.x, 0), r.y = __shfl_sync(0xffffffffu, r.y, 0);
+      r.z = __shfl_sync(0xffffffffu, r.z, 0), r.w = __shfl_sync(0xffffffffu, r.w, 0);
+    } while (r.x == 0);
+    return r.x > 0;
   }
 };
 
@@ -274,10 +290,10 @@ __global__ void __launch_bounds__(512, 1)
   uint64_t* q_full = bars + 0;     // [2] per query tile
   uint64_t* q_empty = bars + 2;    // [2]
   uint64_t* kv_full = bars + 4;    // [2] stage s, in slot s & 1: K of key block s and V of block s - 1
-  uint64_t* kv_ready = bars + 6;   // [2] ... with the hidden V rows cleared and the mask words of block s - 1 written
+  uint64_t* kv_ready = bars + 6;   // [2] MASK: the mask words of block s - 1 are written
   uint64_t* kv_empty = bars + 8;   // [2]
   uint64_t* s_full = bars + 10;    // [2] per query tile
-  uint64_t* p_ready = bars + 12;   // [2]
+  uint64_t* p_ready = bars + 12;   // [2] P is written (softmax group), V and the next K are there (tail warp)
   uint64_t* o_final = bars + 14;   // [2] the tile's last P.V is done
   uint64_t* l_full = bars + 16;    // [2] the tile's maxima and sums are in shared memory
   uint64_t* o_empty = bars + 18;   // [2] accumulator, maxima and sums have been read
@@ -300,7 +316,7 @@ __global__ void __launch_bounds__(512, 1)
       mbar_init(&kv_ready[s], 1);
       mbar_init(&kv_empty[s], 1);
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_ready[s], 128);
+      mbar_init(&p_ready[s], 129);
       mbar_init(&o_final[s], 1);
       mbar_init(&l_full[s], 128);
       mbar_init(&o_empty[s], 4);
@@ -483,65 +499,55 @@ __global__ void __launch_bounds__(512, 1)
       constexpr uint32_t FMT = FP16 ? 0 : 1;
       constexpr uint32_t idesc_pv = make_idesc(128, DK, FMT, FMT, 0, 1);  // B (= V) is MN-major
       // A descriptor holds its address in units of 16 bytes in the low bits, so tiles and k-steps are reached by addition.
-      const uint64_t q_desc = make_desc_k_sw128(smem_u32(smem + CT_Q_OFF));
-      const uint64_t k_desc = make_desc_k_sw128(smem_u32(smem + CT_KV_OFF));
-      const uint64_t v_desc = make_desc_mn_sw128(smem_u32(smem + CT_KV_OFF + 2 * CT_TILE), CT_BOX);
-      CtxItem nt;
+      // The high words (row-group stride, swizzle) of all of them are the same constant.
+      const uint32_t q_desc = static_cast<uint32_t>(make_desc_k_sw128(smem_u32(smem + CT_Q_OFF)));
+      const uint32_t k_desc = static_cast<uint32_t>(make_desc_k_sw128(smem_u32(smem + CT_KV_OFF)));
+      const uint32_t v_desc = static_cast<uint32_t>(make_desc_mn_sw128(smem_u32(smem + CT_KV_OFF + 2 * CT_TILE), CT_BOX));
+      auto desc = [](uint32_t low) { return (make_desc_k_sw128(0) & 0xffffffff00000000ull) | low; };
       int g = 0;
-      uint32_t q_phase = 0, p_phase = 0, o_phase = 3;  // bit per query tile
+      uint32_t q_phase = 0, p_phase = 0;  // bit per query tile
       bool ok = true;
-      // the next item with keys
-      auto next_item = [&](CtxItem& it) {
-        while (items.next(it, ctx, 44))
-          if (it.nb > 0) return true;
-        return false;
-      };
+      
       // one lane: Q.K^T of `cols` columns of ring block gg into S of query tile st; `last`: the item's last block
       auto issue_qk = [&](int st, int gg, int cols, bool last) {
         const uint32_t idesc = make_idesc(128, 0, FMT, FMT, 0, 0) | (static_cast<uint32_t>(cols >> 3) << 17);
-        const uint64_t qd = q_desc + st * (CT_TILE >> 4), kd = k_desc + (gg & 1) * (CT_TILE >> 4);
+        const uint32_t qd = q_desc + st * (CT_TILE >> 4), kd = k_desc + (gg & 1) * (CT_TILE >> 4);
         const uint32_t d = tmem_base + st * 128;
 #pragma unroll
         for (int kk = 0; kk < DK / 16; ++kk) {
           const uint32_t off = ((kk >> 2) * CT_BOX + (kk & 3) * 32) >> 4;
-          umma_f16_ss(d, qd + off, kd + off, idesc, kk ? 1u : 0u);
+          umma_f16_ss(d, desc(qd + off), desc(kd + off), idesc, kk ? 1u : 0u);
         }
         umma_commit(&s_full[st]);
         if (last) umma_commit(&q_empty[st]);
       };
-      auto cols_of = [&](const CtxItem& it, int n) { return (ctx_block_keys(p, it.j0 + n, it.len) + 31) & ~31; };
+      auto cols_of = [](const int4& r, int n) { return n == r.z ? r.w & 0xffff : n + 1 == r.x ? r.w >> 16 : 128; };
       // First scores of an item; its K is already there.
-      auto prime = [&](int st, const CtxItem& it, int gg) {
+      auto prime = [&](int st, const int4& r, int gg) {
         if (!mbar_wait_warp(&q_full[st], (q_phase >> st) & 1, ctx, 45)) return false;
         q_phase ^= 1u << st;
         tc_fence_after();
-        if (elect_one()) issue_qk(st, gg, cols_of(it, 0), it.nb == 1);
-        __syncwarp();
+        if (elect_one()) issue_qk(st, gg, cols_of(r, 0), r.x == 1);
         return true;
       };
-      bool have = next_item(t);
+      int4 t = make_int4(0, 0, 0, 0), nt = t;
+      bool have = items.next_issue(t, ctx, 44);
       if (have) {
-        ok = mbar_wait_warp(&kv_ready[0], 0, ctx, 46) && prime(0, t, 0) && (!t.two(p) || prime(1, t, 0));
+        ok = mbar_wait_warp(&kv_full[0], 0, ctx, 46) && prime(0, t, 0) && (t.y == 1 || prime(1, t, 0));
         if (ok && elect_one()) umma_commit(&kv_empty[0]);
-        __syncwarp();
       }
       while (have && ok) {
-        const int gn = g + t.nb, tiles = t.two(p) ? 2 : 1;
-        const bool have_next = next_item(nt);
-        const int next_tiles = !have_next ? 0 : nt.two(p) ? 2 : 1;
+        const int gn = g + t.x, tiles = t.y;
+        bool have_next = false;
         int cols = cols_of(t, 0);
-        for (; g < gn && ok; ++g) {
-          const bool first = g + t.nb == gn, more = g + 1 < gn;
+        for (int n = 0; n < t.x; ++n, ++g) {
+          const bool more = n + 1 < t.x;
           const int steps = cols >> 4;
-          if (more) cols = cols_of(t, g + 1 - (gn - t.nb));
+          if (more) cols = cols_of(t, n + 1);
           const int slot = (g + 1) & 1;  // stage g + 1: V of this block and K of the next
-          if (!(ok = mbar_wait_warp(&kv_ready[slot], ((g + 1) >> 1) & 1, ctx, 47))) break;
-          const uint64_t vd = v_desc + slot * (CT_TILE >> 4);
+          const uint32_t vd = v_desc + slot * (CT_TILE >> 4);
           for (int st = 0; st < tiles; ++st) {
-            if (first) {  // the accumulator of the tile's previous item has been read
-              if (!(ok = mbar_wait_warp(&o_empty[st], (o_phase >> st) & 1, ctx, 48))) break;
-              o_phase ^= 1u << st;
-            }
+            // P of this block is written, its V and the next K are there, the tile's previous accumulator has been read
             if (!(ok = mbar_wait_warp(&p_ready[st], (p_phase >> st) & 1, ctx, 49))) break;
             p_phase ^= 1u << st;
             tc_fence_after();
@@ -550,21 +556,24 @@ __global__ void __launch_bounds__(512, 1)
               if (steps == 8) {
 #pragma unroll
                 for (int kk = 0; kk < 8; ++kk)
-                  umma_f16_ts(o_tmem, p_tmem + kk * 8, vd + kk * (2048 >> 4), idesc_pv, kk ? 1u : first ? 0u : 1u);
+                  umma_f16_ts(o_tmem, p_tmem + kk * 8, desc(vd + kk * (2048 >> 4)), idesc_pv, kk ? 1u : n ? 1u : 0u);
               } else {
                 for (int kk = 0; kk < steps; ++kk)
-                  umma_f16_ts(o_tmem, p_tmem + kk * 8, vd + kk * (2048 >> 4), idesc_pv, kk ? 1u : first ? 0u : 1u);
+                  umma_f16_ts(o_tmem, p_tmem + kk * 8, desc(vd + kk * (2048 >> 4)), idesc_pv, (kk | n) ? 1u : 0u);
               }
               if (more)
-                issue_qk(st, g + 1, cols, g + 2 == gn);
+                issue_qk(st, g + 1, cols, n + 2 == t.x);
               else
                 umma_commit(&o_final[st]);
             }
             __syncwarp();
-            if (!more && st < next_tiles && !(ok = prime(st, nt, gn))) break;
+            // The next item is looked up behind an item's first products, while the tensor core works on them.
+            if (st == 0 && n == 0) have_next = items.next_issue(nt, ctx, 44);
+            if (!more && have_next && st < nt.y && !(ok = prime(st, nt, gn))) break;
           }
-          if (ok && !more && tiles < next_tiles) ok = prime(1, nt, gn);
-          if (ok && elect_one()) umma_commit(&kv_empty[slot]);
+          if (ok && !more && have_next && tiles < nt.y) ok = prime(1, nt, gn);
+          if (!ok) break;
+          if (elect_one()) umma_commit(&kv_empty[slot]);
           __syncwarp();
         }
         have = have_next;
@@ -573,6 +582,7 @@ __global__ void __launch_bounds__(512, 1)
     } else if (warp == 2) {
       // ------------------------------ tail / mask warp ------------------------------
       int g = 0;
+      uint32_t p_phase = 3;  // bit per query tile
       bool ok = true;
       while (ok && items.next(t, ctx, 52)) {
         // mask bytes of the item's block n, this lane's four keys; loaded one block ahead of their use
@@ -588,10 +598,7 @@ __global__ void __launch_bounds__(512, 1)
         uint8_t m[4];
         if (MASK && t.nb > 0) load_mask(0, m);
         for (int n = 0; n < t.nb; ++n) {
-          if (g == 0) {  // stage 0 has no V
-            if (!(ok = mbar_wait_warp(&kv_full[0], 0, ctx, 62))) break;
-            if (lane == 0) mbar_arrive(&kv_ready[0]);
-          }
+          if (MASK && g == 0 && lane == 0) mbar_arrive(&kv_ready[0]);  // stage 0 has no V and no words
           ++g;  // the stage with this block's V
           const int slot = g & 1;
           const int keys = ctx_block_keys(p, t.j0 + n, t.len);
@@ -623,7 +630,14 @@ __global__ void __launch_bounds__(512, 1)
           }
           if (wrote) fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&kv_ready[slot]);
+          if (MASK && lane == 0) mbar_arrive(&kv_ready[slot]);
+          // one arrival per tile and block: the phase of the block before has to be over
+          for (int st = 0; st < (t.two(p) ? 2 : 1); ++st) {
+            if (!(ok = mbar_wait_warp(&p_ready[st], (p_phase >> st) & 1, ctx, 62))) break;
+            p_phase ^= 1u << st;
+            if (lane == 0) mbar_arrive(&p_ready[st]);
+          }
+          if (!ok) break;
         }
       }
     } else if (warp == 3) {
@@ -640,8 +654,13 @@ __global__ void __launch_bounds__(512, 1)
         const int slot = n % CT_ITEMS;
         if (!mbar_wait_warp(&i_empty[slot], ((n / CT_ITEMS) & 1) ^ 1, ctx, 54)) break;
         if (lane == 0) {
-          ring[slot * 2] = make_int4(t.b, t.hg, t.qp, t.split);
-          ring[slot * 2 + 1] = make_int4(t.first, t.len, t.j0, t.nb);
+          ring[slot * 3] = make_int4(t.b, t.hg, t.qp, t.split);
+          ring[slot * 3 + 1] = make_int4(t.first, t.len, t.j0, t.nb);
+          const int cut = p.n_prefix - 1 - t.j0;  // the prefix's last block, if it is among the item's
+          const int cut_cols = (ctx_block_keys(p, p.n_prefix - 1, t.len) + 31) & ~31;
+          const int last_cols = (ctx_block_keys(p, t.j0 + t.nb - 1, t.len) + 31) & ~31;
+          ring[slot * 3 + 2] = make_int4(end ? -1 : t.nb, t.two(p) ? 2 : 1, p.n_prefix > 0 && cut >= 0 && cut < t.nb ? cut : -1,
+                                         (cut_cols & 0xffff) | last_cols << 16);
           mbar_arrive(&i_full[slot]);
         }
         if (end) break;
@@ -673,8 +692,8 @@ __global__ void __launch_bounds__(512, 1)
         bool part = keys < 128;
         volatile const uint32_t* w = words + ((g + 1) & 1) * 4;
         if (MASK) {
-          // Behind s_full: the scores of block g exist only once stage g was ready, so stage g - 1 was too, and the parity
-          // of stage g + 1 cannot be mistaken for that of stage g - 3 by a group that skipped items.
+          // Behind s_full: the scores of block g follow its K, which came with the V of block g - 1 behind the words of block
+          // g - 2, so the parity of stage g + 1 cannot be mistaken for that of stage g - 3 by a group that skipped items.
           if (!(ok = mbar_wait_warp(&kv_ready[(g + 1) & 1], ((g + 1) >> 1) & 1, ctx, 60))) break;
           part = part || (w[0] & w[1] & w[2] & w[3]) != 0xffffffffu;
         }
@@ -684,11 +703,13 @@ __global__ void __launch_bounds__(512, 1)
           ctx_softmax_full<FP16, DK>(tmem_s, tmem_o, p.c.scale_log2, n == 0, m_used, l);
         tmem_st_wait();
         tc_fence_before();
+        if (n == 0) {  // accumulator, maxima and sums of the previous item have been read
+          if (!(ok = mbar_wait_warp(&o_empty[st], (no & 1) ^ 1, ctx, 61))) break;
+          ++no;
+        }
         mbar_arrive(&p_ready[st]);
       }
       if (!ok) break;
-      if (!(ok = mbar_wait_warp(&o_empty[st], (no & 1) ^ 1, ctx, 61))) break;  // the previous item's have been read
-      ++no;
       ml[st * 128 + row] = make_float2(m_used, l);
       mbar_arrive(&l_full[st]);
     }
@@ -765,3 +786,4 @@ int launch_ctx_tc(const CtxParams& c, int fp16, cudaStream_t st) {
 }
 
 }  // namespace tfb
+
