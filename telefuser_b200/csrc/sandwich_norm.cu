@@ -4,11 +4,16 @@
 // res and y are read once, x and h written once: 8 bytes per element in 16-bit types where the two-kernel chain
 // (rmsnorm_gate_residual, rmsnorm_modulate) moves 10. The second norm reads x as it is stored, so both agree.
 //
-// HBM bound. A thread owns 8 NV fixed columns of every row its CTA walks over, so that what per-sample tables and weights
-// say about those columns (gate * w, w2 * (1 + scale), shift) stays in registers from row to row; reading the fp32 tables
-// again for every row would cost L1 twice the bytes of the row itself. Rows (and per-token tables) arrive through a ring of
-// bulk copies in shared memory, several rows ahead of the two block sums, whose latency would otherwise bound the kernel.
-// Sums, norms and gates are fp32; x and h are rounded once to the activations' type.
+// HBM bound. Rows (and per-token tables) arrive by bulk copies in shared memory; sums, norms and gates are fp32; x and h are
+// rounded once to the activations' type. Two kernels:
+//   warp per row   many rows of a 16-bit type with per-sample tables. The row stays packed in a warp's registers, its two sums
+//                  are shuffles, and no barrier ties warps together. What tables and weights say about a column (gate * w,
+//                  w2 * (1 + scale), shift) lies in shared memory, computed once per CTA: re-reading the fp32 tables
+//                  from global memory for every row would cost L1 twice the bytes of the row itself.
+//   CTA per row    everything else. A thread owns 8 NV fixed columns and keeps what the tables say about them in registers;
+//                  rows come through a ring several rows ahead of the two block sums. Half the latency for a few rows,
+//                  but its barriers and redundant sums take about 3000 instructions per row where the other form takes 1600.
+// 2 x 4224 x 3840 bf16: CTA per row 55 us (four rows behind the same barriers: 76).
 #include <math.h>
 
 #include "tfb_api.h"
@@ -287,8 +292,183 @@ static int launch_snorm_nv(SnormParams& p, int threads, cudaStream_t st) {
   return cudaGetLastError() == cudaSuccess ? TFB_OK : TFB_ERR_LAUNCH;
 }
 
+// ---- warp per row ----
+struct SnormWarpParams {
+  SnormParams s;
+  int per_sample;  // rows of a sample: one row of every table
+  int chunks, per_chunk;
+  int stages;      // rows in flight per warp
+};
+
+template <typename T>
+__device__ __forceinline__ void snorm_unpack(const uint4& u, float (&f)[8]) {
+  Vec8<T> v;
+  v.u = u;
+  v.get(f);
+}
+
+template <typename T, int NVL>
+__global__ void __launch_bounds__(384, 1) sandwich_norm_warp_kernel(const SnormWarpParams wp) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ uint64_t bars[24];
+  __shared__ int abort_flag;
+  const SnormParams& p = wp.s;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+  const int nvec = p.C >> 3;
+  const long b = blockIdx.x / wp.chunks;
+  const long r0 = b * wp.per_sample + static_cast<long>(blockIdx.x % wp.chunks) * wp.per_chunk;
+  const long r1 = min(r0 + wp.per_chunk, (b + 1) * wp.per_sample);
+  const uint32_t row_bytes = p.C * 2;
+  float4* gw = reinterpret_cast<float4*>(smem);  // [2 halves of 8 columns][nvec], as ws and sh: 16-byte steps, no bank conflicts
+  float4* ws = gw + 2 * nvec;
+  float4* sh = ws + 2 * nvec;
+  uint8_t* ring = reinterpret_cast<uint8_t*>(sh + 2 * nvec) + static_cast<long>(warp) * wp.stages * 2 * row_bytes;
+  uint64_t* full = bars + warp * wp.stages;
+  const AbortCtx ctx{&abort_flag, p.status};
+  // one lane: y and res of row r
+  auto fetch = [&](long r, int slot) {
+    uint8_t* dst = ring + slot * 2 * row_bytes;
+    mbar_expect_tx(&full[slot], 2 * row_bytes);
+    bulk_load(dst, static_cast<const T*>(p.y) + r * p.ldy, row_bytes, &full[slot]);
+    bulk_load(dst + row_bytes, static_cast<const T*>(p.res) + r * p.ldr, row_bytes, &full[slot]);
+  };
+  if (lane == 0) {
+    for (int s = 0; s < wp.stages; ++s) mbar_init(&full[s], 1);
+    mbar_fence_init();
+    for (int s = 0; s < wp.stages; ++s)
+      if (r0 + warp + static_cast<long>(s) * nw < r1) fetch(r0 + warp + static_cast<long>(s) * nw, s);
+    if (warp == 0) abort_flag = 0;
+  }
+  for (int vi = threadIdx.x; vi < nvec; vi += blockDim.x) {
+    const int col = vi * 8;
+    float a[8], t[8];
+    snorm_weight<T>(p.post ? p.w : nullptr, p.w_f32, col, a);
+    if (p.gate) {
+      snorm_table(p.gate, r0 / p.rpg * p.ldg + col, t);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a[e] *= p.tanh_gate ? snorm_tanh(t[e]) : t[e];
+    }
+    gw[vi] = make_float4(a[0], a[1], a[2], a[3]), gw[nvec + vi] = make_float4(a[4], a[5], a[6], a[7]);
+    snorm_weight<T>(p.w2, p.w_f32, col, a);
+    if (p.scale) {
+      snorm_table(p.scale, r0 / p.rpc * p.ldc + col, t);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a[e] *= 1.f + t[e];
+    }
+    ws[vi] = make_float4(a[0], a[1], a[2], a[3]), ws[nvec + vi] = make_float4(a[4], a[5], a[6], a[7]);
+    snorm_table(p.shift, p.shift ? r0 / p.rps * p.lds + col : 0, t);
+    sh[vi] = make_float4(t[0], t[1], t[2], t[3]), sh[nvec + vi] = make_float4(t[4], t[5], t[6], t[7]);
+  }
+  __syncthreads();
+
+  const float inv_c = 1.f / p.C;
+  int slot = 0;
+  uint32_t phase = 0;
+  for (long r = r0 + warp; r < r1; r += nw) {
+    // after an expired wait (recorded in the status word) the warp goes on with what is there
+    mbar_wait_warp(&full[slot], phase, ctx, 71);
+    const uint4* sy = reinterpret_cast<const uint4*>(ring + slot * 2 * row_bytes);
+    const uint4* sr = reinterpret_cast<const uint4*>(ring + slot * 2 * row_bytes + row_bytes);
+    uint4 row[NVL];  // y, then x as stored
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < NVL; ++i) {
+      const int vi = lane + i * 32;
+      if (vi < nvec) {
+        row[i] = sy[vi];
+        float f[8];
+        snorm_unpack<T>(row[i], f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss += f[e] * f[e];
+      }
+    }
+    const float rstd = p.post ? rsqrtf(warp_sum(ss) * inv_c + p.eps) : 1.f;
+    ss = 0.f;
+    uint4* xo = reinterpret_cast<uint4*>(static_cast<T*>(p.x) + r * p.C);
+#pragma unroll
+    for (int i = 0; i < NVL; ++i) {
+      const int vi = lane + i * 32;
+      if (vi < nvec) {
+        float y[8], f[8];
+        snorm_unpack<T>(row[i], y);
+        snorm_unpack<T>(sr[vi], f);
+        const float4 g0 = gw[vi], g1 = gw[nvec + vi];
+        const float g[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] += y[e] * rstd * g[e];
+        Vec8<T> v;
+        v.put(f);
+        row[i] = v.u;
+        xo[vi] = v.u;
+        v.get(f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss += f[e] * f[e];
+      }
+    }
+    __syncwarp();
+    if (lane == 0 && r + static_cast<long>(wp.stages) * nw < r1) fetch(r + static_cast<long>(wp.stages) * nw, slot);
+    if (++slot == wp.stages) slot = 0, phase ^= 1;
+    const float rstd2 = rsqrtf(warp_sum(ss) * inv_c + p.eps);
+    uint4* ho = reinterpret_cast<uint4*>(static_cast<T*>(p.h) + r * p.C);
+#pragma unroll
+    for (int i = 0; i < NVL; ++i) {
+      const int vi = lane + i * 32;
+      if (vi < nvec) {
+        float f[8];
+        snorm_unpack<T>(row[i], f);
+        const float4 w0 = ws[vi], w1 = ws[nvec + vi], s0 = sh[vi], s1 = sh[nvec + vi];
+        const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w}, s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = f[e] * rstd2 * w[e] + s[e];
+        Vec8<T> v;
+        v.put(f);
+        ho[vi] = v.u;
+      }
+    }
+  }
+}
+
+template <typename T, int NVL>
+static int launch_snorm_warp(const SnormParams& p, long per_sample, cudaStream_t st) {
+  static bool attr_set[TFB_MAX_DEVICES] = {false};
+  constexpr int SMEM = 220 * 1024;
+  auto kern = &sandwich_norm_warp_kernel<T, NVL>;
+  if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), SMEM, attr_set)) return rc;
+  SnormWarpParams wp;
+  wp.s = p;
+  wp.per_sample = static_cast<int>(per_sample);
+  const int tables = 3 * 4 * p.C, stage = 4 * p.C;
+  // twelve warps, two rows each if they fit, else one
+  int fit = (SMEM - tables) / stage;
+  wp.stages = fit >= 24 ? 2 : 1;
+  const int warps = fit / wp.stages < 12 ? fit / wp.stages : 12;
+  const long samples = p.rows / per_sample;
+  long chunks = sm_count() / samples;  // one CTA per SM
+  if (chunks < 1) chunks = 1;
+  if (chunks > (per_sample + warps - 1) / warps) chunks = (per_sample + warps - 1) / warps;
+  wp.per_chunk = static_cast<int>((per_sample + chunks - 1) / chunks);
+  wp.chunks = static_cast<int>((per_sample + wp.per_chunk - 1) / wp.per_chunk);
+  kern<<<static_cast<int>(samples * wp.chunks), warps * 32, tables + warps * wp.stages * stage, st>>>(wp);
+  return cudaGetLastError() == cudaSuccess ? TFB_OK : TFB_ERR_LAUNCH;
+}
+
+// Warp per row: per-sample tables, 16-bit rows of up to 5120 columns (so that six rows and the tables fit), and rows enough
+// for eight warps on every SM.
+template <typename T>
+static bool snorm_by_warps(const SnormParams& p) {
+  return sizeof(T) == 2 && !p.token && p.C <= 5120 && p.rows >= 8L * sm_count() && p.rows <= 0x7fffffffL;
+}
+
 template <typename T>
 static int launch_snorm(SnormParams& p, cudaStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (snorm_by_warps<T>(p)) {
+      if (p.C <= 1024) return launch_snorm_warp<T, 4>(p, p.rp, st);
+      if (p.C <= 2048) return launch_snorm_warp<T, 8>(p, p.rp, st);
+      if (p.C <= 4096) return launch_snorm_warp<T, 16>(p, p.rp, st);
+      return launch_snorm_warp<T, 20>(p, p.rp, st);
+    }
+  }
   const int nvec = p.C / 8;
   const int nv = nvec > 512 ? 2 : 1;
   const int threads = ((nvec + nv - 1) / nv + 31) / 32 * 32;

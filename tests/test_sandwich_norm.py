@@ -73,7 +73,7 @@ gpu = pytest.mark.gpu
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("tables", ["sample", "token", "one"])
-@pytest.mark.parametrize("B,S,C", [(1, 1, 8), (1, 3, 2048), (2, 77, 3840), (3, 5, 40), (2, 1001, 264), (1, 300, 4104), (2, 9, 8192)])
+@pytest.mark.parametrize("B,S,C", [(1, 1, 8), (1, 3, 2048), (2, 77, 3840), (3, 5, 40), (2, 1001, 264), (1, 300, 4104), (2, 9, 8192), (2, 700, 3840), (3, 500, 72), (1, 1300, 5120), (40, 33, 2048)])
 def test_matches_the_definition(B, S, C, tables, dtype):
     a = inputs(B, S, C, dtype, "cuda", tables)
     check(*TF.rmsnorm_gate_residual_modulate(**a), a)
