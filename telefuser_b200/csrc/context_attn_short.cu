@@ -9,10 +9,11 @@
 // this kernel's figure for 21 frames of 1560 tokens x 40 heads against 32 keys.)
 // Coalescing comes from permuting indexes: a lane loads and stores whole 16-byte pieces of a row, and the copies of K and V
 // in shared memory have their channels reordered to match what the fragments then hold:
-//   Q.K^T  lane (n, c) = (lane / 4, lane % 4) holds channels 32 i + 8 c .. + 7 of row n, i.e. of k-step u = 0, 1 the pairs
-//          4 u + 2 h (h = 0, 1): K stores channel 32 i + 8 c + 4 u + 2 h + e at position 32 i + 16 u + 8 h + 2 c + e
-//   P.V    column 2 c + e of tile t is channel 64 blk + 32 e + 8 c + t, so that the four lanes of a row store 64 bytes next to
-//          each other: V stores that channel at position 64 blk + 8 t + 2 c + e
+//   Q.K^T  lane (n, c) = (lane / 4, lane % 4) holds channels 32 i + 8 c .. + 7 of row n; it feeds pair w (channels 2 w, 2 w + 1
+//          of them) into half w % 2 of k-step w / 2
+//   P.V    columns 2 c, 2 c + 1 of MMA 4 i + w are the same two channels, so a lane ends up with 16 bytes of its row and the
+//          four lanes of a row with 64 bytes next to each other
+// Both want channel 32 i + 8 c + 2 w + e at position 32 i + 8 w + 2 c + e.
 // Hidden keys are zeros in both copies and their scores become -inf, so what lies there does not matter.
 #include "context_attn.cuh"
 
@@ -91,13 +92,11 @@ __global__ void __launch_bounds__(CS_WARPS * 32, STEPS == 2 ? 5 : 4) ctx_short_k
       kw = __ldg(reinterpret_cast<const uint4*>(kb + static_cast<long>(key) * p.k_ss + ch));
       vw = __ldg(reinterpret_cast<const uint4*>(vb + static_cast<long>(key) * p.v_ss + ch));
     }
-    uint16_t* kd = s_k + key * LD + (ch & ~31) + (ch >> 3 & 3) * 2;
-    uint16_t* vd = s_v + key * LD + (ch & ~63) + (ch >> 3 & 3) * 2 + (ch >> 5 & 1);
+    const int at = key * LD + (ch & ~31) + (ch >> 3 & 3) * 2;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {  // word w: channels ch + 2 w, + 1; u = w / 2, h = w % 2
-      *reinterpret_cast<uint32_t*>(kd + (w >> 1) * 16 + (w & 1) * 8) = (&kw.x)[w];
-      vd[(2 * w) * 8] = static_cast<uint16_t>((&vw.x)[w] & 0xffffu);
-      vd[(2 * w + 1) * 8] = static_cast<uint16_t>((&vw.x)[w] >> 16);
+    for (int w = 0; w < 4; ++w) {
+      *reinterpret_cast<uint32_t*>(s_k + at + w * 8) = (&kw.x)[w];
+      *reinterpret_cast<uint32_t*>(s_v + at + w * 8) = (&vw.x)[w];
     }
   }
   // hidden keys among this lane's score columns 16 step + 8 t + 2 c + e, as bits 4 step + 2 t + e
@@ -206,12 +205,12 @@ __global__ void __launch_bounds__(CS_WARPS * 32, STEPS == 2 ? 5 : 4) ctx_short_k
 #pragma unroll
       for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int d = blk * 64 + 32 * e + 8 * c;
-          uint4 w;
+        for (int h = 0; h < 2; ++h) {
+          const int d = blk * 64 + 32 * h + 8 * c;
+          uint4 v;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) (&w.x)[x] = ctx_pack2<FP16>(o[2 * x][r * 2 + e] * inv[r], o[2 * x + 1][r * 2 + e] * inv[r]);
-          if (row_ok[r] && d < p.D) *reinterpret_cast<uint4*>(ob + row_at[r] + d) = w;
+          for (int w = 0; w < 4; ++w) (&v.x)[w] = ctx_pack2<FP16>(o[h * 4 + w][r * 2] * inv[r], o[h * 4 + w][r * 2 + 1] * inv[r]);
+          if (row_ok[r] && d < p.D) *reinterpret_cast<uint4*>(ob + row_at[r] + d) = v;
         }
     }
   }

@@ -300,11 +300,36 @@ struct SnormWarpParams {
   int stages;      // rows in flight per warp
 };
 
+// Two 16-bit values as packed fp32 and back.
 template <typename T>
-__device__ __forceinline__ void snorm_unpack(const uint4& u, float (&f)[8]) {
-  Vec8<T> v;
-  v.u = u;
-  v.get(f);
+__device__ __forceinline__ uint64_t snorm_unpack2(uint32_t v);
+template <>
+__device__ __forceinline__ uint64_t snorm_unpack2<__nv_bfloat16>(uint32_t v) {
+  return f2_pack(bf16_lo(v), bf16_hi(v));
+}
+template <>
+__device__ __forceinline__ uint64_t snorm_unpack2<__half>(uint32_t v) {
+  const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&v));
+  return f2_pack(t.x, t.y);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t snorm_pack2(uint64_t v);
+template <>
+__device__ __forceinline__ uint32_t snorm_pack2<__nv_bfloat16>(uint64_t v) {
+  float a, b;
+  f2_unpack(v, a, b);
+  return pack_bf16x2(a, b);
+}
+template <>
+__device__ __forceinline__ uint32_t snorm_pack2<__half>(uint64_t v) {
+  float a, b;
+  f2_unpack(v, a, b);
+  return pack_f16x2(a, b);
+}
+__device__ __forceinline__ float snorm_total(const uint64_t (&s)[4]) {
+  float a, b;
+  f2_unpack(f2_add(f2_add(s[0], s[1]), f2_add(s[2], s[3])), a, b);
+  return warp_sum(a + b);
 }
 
 template <typename T, int NVL>
@@ -319,9 +344,10 @@ __global__ void __launch_bounds__(384, 1) sandwich_norm_warp_kernel(const SnormW
   const long r0 = b * wp.per_sample + static_cast<long>(blockIdx.x % wp.chunks) * wp.per_chunk;
   const long r1 = min(r0 + wp.per_chunk, (b + 1) * wp.per_sample);
   const uint32_t row_bytes = p.C * 2;
-  float4* gw = reinterpret_cast<float4*>(smem);  // [2 halves of 8 columns][nvec], as ws and sh: 16-byte steps, no bank conflicts
-  float4* ws = gw + 2 * nvec;
-  float4* sh = ws + 2 * nvec;
+  // packed fp32, [2 halves of 8 columns][nvec]: 16-byte steps from lane to lane, no bank conflicts
+  ulonglong2* gw = reinterpret_cast<ulonglong2*>(smem);
+  ulonglong2* ws = gw + 2 * nvec;
+  ulonglong2* sh = ws + 2 * nvec;
   uint8_t* ring = reinterpret_cast<uint8_t*>(sh + 2 * nvec) + static_cast<long>(warp) * wp.stages * 2 * row_bytes;
   uint64_t* full = bars + warp * wp.stages;
   const AbortCtx ctx{&abort_flag, p.status};
@@ -348,16 +374,19 @@ __global__ void __launch_bounds__(384, 1) sandwich_norm_warp_kernel(const SnormW
 #pragma unroll
       for (int e = 0; e < 8; ++e) a[e] *= p.tanh_gate ? snorm_tanh(t[e]) : t[e];
     }
-    gw[vi] = make_float4(a[0], a[1], a[2], a[3]), gw[nvec + vi] = make_float4(a[4], a[5], a[6], a[7]);
+    gw[vi] = make_ulonglong2(f2_pack(a[0], a[1]), f2_pack(a[2], a[3]));
+    gw[nvec + vi] = make_ulonglong2(f2_pack(a[4], a[5]), f2_pack(a[6], a[7]));
     snorm_weight<T>(p.w2, p.w_f32, col, a);
     if (p.scale) {
       snorm_table(p.scale, r0 / p.rpc * p.ldc + col, t);
 #pragma unroll
       for (int e = 0; e < 8; ++e) a[e] *= 1.f + t[e];
     }
-    ws[vi] = make_float4(a[0], a[1], a[2], a[3]), ws[nvec + vi] = make_float4(a[4], a[5], a[6], a[7]);
+    ws[vi] = make_ulonglong2(f2_pack(a[0], a[1]), f2_pack(a[2], a[3]));
+    ws[nvec + vi] = make_ulonglong2(f2_pack(a[4], a[5]), f2_pack(a[6], a[7]));
     snorm_table(p.shift, p.shift ? r0 / p.rps * p.lds + col : 0, t);
-    sh[vi] = make_float4(t[0], t[1], t[2], t[3]), sh[nvec + vi] = make_float4(t[4], t[5], t[6], t[7]);
+    sh[vi] = make_ulonglong2(f2_pack(t[0], t[1]), f2_pack(t[2], t[3]));
+    sh[nvec + vi] = make_ulonglong2(f2_pack(t[4], t[5]), f2_pack(t[6], t[7]));
   }
   __syncthreads();
 
@@ -370,59 +399,57 @@ __global__ void __launch_bounds__(384, 1) sandwich_norm_warp_kernel(const SnormW
     const uint4* sy = reinterpret_cast<const uint4*>(ring + slot * 2 * row_bytes);
     const uint4* sr = reinterpret_cast<const uint4*>(ring + slot * 2 * row_bytes + row_bytes);
     uint4 row[NVL];  // y, then x as stored
-    float ss = 0.f;
+    uint64_t ss[4] = {0ull, 0ull, 0ull, 0ull};  // packed fp32, four chains
 #pragma unroll
     for (int i = 0; i < NVL; ++i) {
       const int vi = lane + i * 32;
       if (vi < nvec) {
         row[i] = sy[vi];
-        float f[8];
-        snorm_unpack<T>(row[i], f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss += f[e] * f[e];
+        for (int e = 0; e < 4; ++e) {
+          const uint64_t y = snorm_unpack2<T>((&row[i].x)[e]);
+          ss[e] = f2_fma(y, y, ss[e]);
+        }
       }
     }
-    const float rstd = p.post ? rsqrtf(warp_sum(ss) * inv_c + p.eps) : 1.f;
-    ss = 0.f;
+    const float rstd = p.post ? rsqrtf(snorm_total(ss) * inv_c + p.eps) : 1.f;
+    const uint64_t rstd_2 = f2_pack(rstd, rstd);
+    ss[0] = ss[1] = ss[2] = ss[3] = 0ull;
     uint4* xo = reinterpret_cast<uint4*>(static_cast<T*>(p.x) + r * p.C);
 #pragma unroll
     for (int i = 0; i < NVL; ++i) {
       const int vi = lane + i * 32;
       if (vi < nvec) {
-        float y[8], f[8];
-        snorm_unpack<T>(row[i], y);
-        snorm_unpack<T>(sr[vi], f);
-        const float4 g0 = gw[vi], g1 = gw[nvec + vi];
-        const float g[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
+        const uint4 rv = sr[vi];
+        const ulonglong2 g0 = gw[vi], g1 = gw[nvec + vi];
+        const uint64_t g[4] = {g0.x, g0.y, g1.x, g1.y};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] += y[e] * rstd * g[e];
-        Vec8<T> v;
-        v.put(f);
-        row[i] = v.u;
-        xo[vi] = v.u;
-        v.get(f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss += f[e] * f[e];
+        for (int e = 0; e < 4; ++e) {
+          uint32_t& v = (&row[i].x)[e];
+          v = snorm_pack2<T>(f2_fma(snorm_unpack2<T>(v), f2_mul(g[e], rstd_2), snorm_unpack2<T>((&rv.x)[e])));
+          const uint64_t x = snorm_unpack2<T>(v);
+          ss[e] = f2_fma(x, x, ss[e]);
+        }
+        xo[vi] = row[i];
       }
     }
     __syncwarp();
     if (lane == 0 && r + static_cast<long>(wp.stages) * nw < r1) fetch(r + static_cast<long>(wp.stages) * nw, slot);
     if (++slot == wp.stages) slot = 0, phase ^= 1;
-    const float rstd2 = rsqrtf(warp_sum(ss) * inv_c + p.eps);
+    const float rstd2 = rsqrtf(snorm_total(ss) * inv_c + p.eps);
+    const uint64_t rstd2_2 = f2_pack(rstd2, rstd2);
     uint4* ho = reinterpret_cast<uint4*>(static_cast<T*>(p.h) + r * p.C);
 #pragma unroll
     for (int i = 0; i < NVL; ++i) {
       const int vi = lane + i * 32;
       if (vi < nvec) {
-        float f[8];
-        snorm_unpack<T>(row[i], f);
-        const float4 w0 = ws[vi], w1 = ws[nvec + vi], s0 = sh[vi], s1 = sh[nvec + vi];
-        const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w}, s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+        const ulonglong2 w0 = ws[vi], w1 = ws[nvec + vi], s0 = sh[vi], s1 = sh[nvec + vi];
+        const uint64_t w[4] = {w0.x, w0.y, w1.x, w1.y}, s[4] = {s0.x, s0.y, s1.x, s1.y};
+        uint4 v;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = f[e] * rstd2 * w[e] + s[e];
-        Vec8<T> v;
-        v.put(f);
-        ho[vi] = v.u;
+        for (int e = 0; e < 4; ++e)
+          (&v.x)[e] = snorm_pack2<T>(f2_fma(f2_mul(snorm_unpack2<T>((&row[i].x)[e]), rstd2_2), w[e], s[e]));
+        ho[vi] = v;
       }
     }
   }
