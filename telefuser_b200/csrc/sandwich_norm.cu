@@ -335,7 +335,7 @@ __device__ __forceinline__ float snorm_total(const uint64_t (&s)[4]) {
 template <typename T, int NVL>
 __global__ void __launch_bounds__(384, 1) sandwich_norm_warp_kernel(const SnormWarpParams wp) {
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ uint64_t bars[24];
+  __shared__ uint64_t bars[24], tables_full;
   __shared__ int abort_flag;
   const SnormParams& p = wp.s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
@@ -343,12 +343,14 @@ __global__ void __launch_bounds__(384, 1) sandwich_norm_warp_kernel(const SnormW
   const long b = blockIdx.x / wp.chunks;
   const long r0 = b * wp.per_sample + static_cast<long>(blockIdx.x % wp.chunks) * wp.per_chunk;
   const long r1 = min(r0 + wp.per_chunk, (b + 1) * wp.per_sample);
-  const uint32_t row_bytes = p.C * 2;
-  // packed fp32, [2 halves of 8 columns][nvec]: 16-byte steps from lane to lane, no bank conflicts
-  ulonglong2* gw = reinterpret_cast<ulonglong2*>(smem);
-  ulonglong2* ws = gw + 2 * nvec;
-  ulonglong2* sh = ws + 2 * nvec;
-  uint8_t* ring = reinterpret_cast<uint8_t*>(sh + 2 * nvec) + static_cast<long>(warp) * wp.stages * 2 * row_bytes;
+  const uint32_t row_bytes = p.C * 2, w_bytes = p.C * (p.w_f32 ? 4 : 2);
+  // gate, scale, shift as they come, then in their place gate * w, w2 * (1 + scale), shift: fp32, 32 bytes per 8 columns, the
+  // two halves of every second group of four swapped, so that lanes reading one half each meet no bank twice
+  float* gw = reinterpret_cast<float*>(smem);
+  float *ws = gw + p.C, *sh = ws + p.C;
+  uint8_t* raw_w = smem + 12 * p.C;
+  uint8_t* raw_w2 = raw_w + w_bytes;
+  uint8_t* ring = raw_w2 + w_bytes + static_cast<long>(warp) * wp.stages * 2 * row_bytes;
   uint64_t* full = bars + warp * wp.stages;
   const AbortCtx ctx{&abort_flag, p.status};
   // one lane: y and res of row r
@@ -358,35 +360,64 @@ __global__ void __launch_bounds__(384, 1) sandwich_norm_warp_kernel(const SnormW
     bulk_load(dst, static_cast<const T*>(p.y) + r * p.ldy, row_bytes, &full[slot]);
     bulk_load(dst + row_bytes, static_cast<const T*>(p.res) + r * p.ldr, row_bytes, &full[slot]);
   };
+  // Tables and weights first: behind the first rows of every CTA, 25 MB, they came 8 us later.
+  if (threadIdx.x == 0) {
+    mbar_init(&tables_full, 1);
+    abort_flag = 0;
+    mbar_fence_init();
+    const bool post_w = p.post && p.w;
+    mbar_expect_tx(&tables_full, p.C * 4 * ((p.gate != nullptr) + (p.scale != nullptr) + (p.shift != nullptr)) +
+                                     w_bytes * (post_w + (p.w2 != nullptr)));
+    if (p.gate) bulk_load(gw, p.gate + r0 / p.rpg * p.ldg, p.C * 4, &tables_full);
+    if (p.scale) bulk_load(ws, p.scale + r0 / p.rpc * p.ldc, p.C * 4, &tables_full);
+    if (p.shift) bulk_load(sh, p.shift + r0 / p.rps * p.lds, p.C * 4, &tables_full);
+    if (post_w) bulk_load(raw_w, p.w, w_bytes, &tables_full);
+    if (p.w2) bulk_load(raw_w2, p.w2, w_bytes, &tables_full);
+  }
   if (lane == 0) {
     for (int s = 0; s < wp.stages; ++s) mbar_init(&full[s], 1);
     mbar_fence_init();
+  }
+  __syncthreads();
+  if (lane == 0)
     for (int s = 0; s < wp.stages; ++s)
       if (r0 + warp + static_cast<long>(s) * nw < r1) fetch(r0 + warp + static_cast<long>(s) * nw, s);
-    if (warp == 0) abort_flag = 0;
-  }
+  mbar_wait(&tables_full, 0, ctx, 72);
+  // Four columns a step, each thread its own 8 in place. Kept small on purpose: unrolled, with a tanh per column, this was
+  // mostly the fetching of instructions.
+#pragma unroll 1
   for (int vi = threadIdx.x; vi < nvec; vi += blockDim.x) {
-    const int col = vi * 8;
-    float a[8], t[8];
-    snorm_weight<T>(p.post ? p.w : nullptr, p.w_f32, col, a);
-    if (p.gate) {
-      snorm_table(p.gate, r0 / p.rpg * p.ldg + col, t);
+    float4 g[2], c[2], h[2];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) a[e] *= p.tanh_gate ? snorm_tanh(t[e]) : t[e];
+    for (int q = 0; q < 2; ++q) {
+      const int col = vi * 8 + q * 4;
+      auto weight = [&](const uint8_t* w) {
+        if (p.w_f32) return *reinterpret_cast<const float4*>(w + col * 4);
+        const uint2 u = *reinterpret_cast<const uint2*>(w + col * 2);
+        float4 f;
+        f2_unpack(snorm_unpack2<T>(u.x), f.x, f.y);
+        f2_unpack(snorm_unpack2<T>(u.y), f.z, f.w);
+        return f;
+      };
+      const float4 one = make_float4(1.f, 1.f, 1.f, 1.f), zero = make_float4(0.f, 0.f, 0.f, 0.f);
+      const float4 w = p.post && p.w ? weight(raw_w) : one, w2 = p.w2 ? weight(raw_w2) : one;
+      g[q] = p.gate ? *reinterpret_cast<const float4*>(gw + col) : one;
+      c[q] = p.scale ? *reinterpret_cast<const float4*>(ws + col) : zero;
+      h[q] = p.shift ? *reinterpret_cast<const float4*>(sh + col) : zero;
+      if (p.gate && p.tanh_gate) {
+#pragma unroll 1
+        for (int e = 0; e < 4; ++e) g[q] = make_float4(g[q].y, g[q].z, g[q].w, snorm_tanh(g[q].x));
+      }
+      g[q] = make_float4(w.x * g[q].x, w.y * g[q].y, w.z * g[q].z, w.w * g[q].w);
+      c[q] = make_float4(w2.x * (1.f + c[q].x), w2.y * (1.f + c[q].y), w2.z * (1.f + c[q].z), w2.w * (1.f + c[q].w));
     }
-    gw[vi] = make_ulonglong2(f2_pack(a[0], a[1]), f2_pack(a[2], a[3]));
-    gw[nvec + vi] = make_ulonglong2(f2_pack(a[4], a[5]), f2_pack(a[6], a[7]));
-    snorm_weight<T>(p.w2, p.w_f32, col, a);
-    if (p.scale) {
-      snorm_table(p.scale, r0 / p.rpc * p.ldc + col, t);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) a[e] *= 1.f + t[e];
+    for (int q = 0; q < 2; ++q) {
+      const int at = vi * 2 + (q ^ (vi >> 2 & 1));
+      reinterpret_cast<float4*>(gw)[at] = g[q];
+      reinterpret_cast<float4*>(ws)[at] = c[q];
+      reinterpret_cast<float4*>(sh)[at] = h[q];
     }
-    ws[vi] = make_ulonglong2(f2_pack(a[0], a[1]), f2_pack(a[2], a[3]));
-    ws[nvec + vi] = make_ulonglong2(f2_pack(a[4], a[5]), f2_pack(a[6], a[7]));
-    snorm_table(p.shift, p.shift ? r0 / p.rps * p.lds + col : 0, t);
-    sh[vi] = make_ulonglong2(f2_pack(t[0], t[1]), f2_pack(t[2], t[3]));
-    sh[nvec + vi] = make_ulonglong2(f2_pack(t[4], t[5]), f2_pack(t[6], t[7]));
   }
   __syncthreads();
 
@@ -421,7 +452,8 @@ __global__ void __launch_bounds__(384, 1) sandwich_norm_warp_kernel(const SnormW
       const int vi = lane + i * 32;
       if (vi < nvec) {
         const uint4 rv = sr[vi];
-        const ulonglong2 g0 = gw[vi], g1 = gw[nvec + vi];
+        const int at = vi * 2 + (vi >> 2 & 1);  // of the first half; the second is next to it
+        const ulonglong2 g0 = reinterpret_cast<const ulonglong2*>(gw)[at], g1 = reinterpret_cast<const ulonglong2*>(gw)[at ^ 1];
         const uint64_t g[4] = {g0.x, g0.y, g1.x, g1.y};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -443,7 +475,9 @@ __global__ void __launch_bounds__(384, 1) sandwich_norm_warp_kernel(const SnormW
     for (int i = 0; i < NVL; ++i) {
       const int vi = lane + i * 32;
       if (vi < nvec) {
-        const ulonglong2 w0 = ws[vi], w1 = ws[nvec + vi], s0 = sh[vi], s1 = sh[nvec + vi];
+        const int at = vi * 2 + (vi >> 2 & 1);
+        const ulonglong2 w0 = reinterpret_cast<const ulonglong2*>(ws)[at], w1 = reinterpret_cast<const ulonglong2*>(ws)[at ^ 1];
+        const ulonglong2 s0 = reinterpret_cast<const ulonglong2*>(sh)[at], s1 = reinterpret_cast<const ulonglong2*>(sh)[at ^ 1];
         const uint64_t w[4] = {w0.x, w0.y, w1.x, w1.y}, s[4] = {s0.x, s0.y, s1.x, s1.y};
         uint4 v;
 #pragma unroll
@@ -464,7 +498,7 @@ static int launch_snorm_warp(const SnormParams& p, long per_sample, cudaStream_t
   SnormWarpParams wp;
   wp.s = p;
   wp.per_sample = static_cast<int>(per_sample);
-  const int tables = 3 * 4 * p.C, stage = 4 * p.C;
+  const int tables = 3 * 4 * p.C + 2 * p.C * (p.w_f32 ? 4 : 2), stage = 4 * p.C;
   // twelve warps, two rows each if they fit, else one
   int fit = (SMEM - tables) / stage;
   wp.stages = fit >= 24 ? 2 : 1;
