@@ -540,33 +540,34 @@ static int launch_snorm(SnormParams& p, cudaStream_t st) {
 
 using namespace tfb;
 
-extern "C" int tfb_sandwich_norm(const void* res, long ldr, const void* y, long ldy, void* x, void* h, long rows, int C,
-                                 float eps, int dtype, int w_f32, const void* w, const void* w2, const float* gate, long ldg,
-                                 long rpg, const float* shift, long lds, long rps, const float* scale, long ldc, long rpc,
-                                 int post, int tanh_gate, void* stream) {
-  if (rows <= 0) return TFB_OK;
-  const long align = dtype == 2 ? 4 : 8;
-  if (C < 8 || C % 8 || C > 8192 || ldr % align || ldy % align || dtype < 0 || dtype > 2) return TFB_ERR_BAD_SHAPE;
-  if ((gate && (ldg % 4 || rpg < 1)) || (shift && (lds % 4 || rps < 1)) || (scale && (ldc % 4 || rpc < 1))) return TFB_ERR_BAD_SHAPE;
+extern "C" int tfb_sandwich_norm(const tfb_sandwich_norm_args* a, void* stream) {
+  if (!a) return TFB_ERR_BAD_SHAPE;
+  if (a->rows <= 0) return TFB_OK;
+  const long align = a->dtype == 2 ? 4 : 8;
+  if (a->C < 8 || a->C % 8 || a->C > 8192 || a->ldr % align || a->ldy % align || a->dtype < 0 || a->dtype > 2) return TFB_ERR_BAD_SHAPE;
+  if (!a->res || !a->y || !a->x || !a->h) return TFB_ERR_BAD_SHAPE;
+  if ((a->gate && (a->ldg % 4 || a->rpg < 1)) || (a->shift && (a->lds % 4 || a->rps < 1)) || (a->scale && (a->ldc % 4 || a->rpc < 1)))
+    return TFB_ERR_BAD_SHAPE;
   uintptr_t any = 0;
-  for (const void* q : {res, y, static_cast<const void*>(x), static_cast<const void*>(h), w, w2,
-                        static_cast<const void*>(gate), static_cast<const void*>(shift), static_cast<const void*>(scale)})
+  for (const void* q : {a->res, a->y, static_cast<const void*>(a->x), static_cast<const void*>(a->h), a->w, a->w2,
+                        static_cast<const void*>(a->gate), static_cast<const void*>(a->shift), static_cast<const void*>(a->scale)})
     any |= reinterpret_cast<uintptr_t>(q);
   if (any & 15) return TFB_ERR_BAD_SHAPE;
   SnormParams p;
-  p.res = res, p.y = y, p.x = x, p.h = h, p.ldr = ldr, p.ldy = ldy, p.rows = rows, p.C = C, p.w_f32 = w_f32, p.post = post;
-  p.tanh_gate = tanh_gate, p.eps = eps, p.w = w, p.w2 = w2, p.gate = gate, p.shift = shift, p.scale = scale;
-  p.ldg = ldg, p.rpg = rpg, p.lds = lds, p.rps = rps, p.ldc = ldc, p.rpc = rpc;
+  p.res = a->res, p.y = a->y, p.x = a->x, p.h = a->h, p.ldr = a->ldr, p.ldy = a->ldy, p.rows = a->rows, p.C = a->C;
+  p.w_f32 = a->w_f32, p.post = a->post, p.tanh_gate = a->tanh_gate, p.eps = a->eps, p.w = a->w, p.w2 = a->w2;
+  p.gate = a->gate, p.shift = a->shift, p.scale = a->scale;
+  p.ldg = a->ldg, p.rpg = a->rpg, p.lds = a->lds, p.rps = a->rps, p.ldc = a->ldc, p.rpc = a->rpc;
   // Tables that change from row to row go through the ring; the others change together where they change at all (one row
   // per sample or one in all).
-  p.token = (gate && rpg == 1 && ldg ? 1 : 0) | (shift && rps == 1 && lds ? 2 : 0) | (scale && rpc == 1 && ldc ? 4 : 0);
-  p.rp = rows;
-  if (gate && !(p.token & 1) && rpg < p.rp) p.rp = rpg;
-  if (shift && !(p.token & 2) && rps < p.rp) p.rp = rps;
-  if (scale && !(p.token & 4) && rpc < p.rp) p.rp = rpc;
+  p.token = (p.gate && p.rpg == 1 && p.ldg ? 1 : 0) | (p.shift && p.rps == 1 && p.lds ? 2 : 0) | (p.scale && p.rpc == 1 && p.ldc ? 4 : 0);
+  p.rp = p.rows;
+  if (p.gate && !(p.token & 1) && p.rpg < p.rp) p.rp = p.rpg;
+  if (p.shift && !(p.token & 2) && p.rps < p.rp) p.rp = p.rps;
+  if (p.scale && !(p.token & 4) && p.rpc < p.rp) p.rp = p.rpc;
   p.status = status_word();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == 0) return launch_snorm<__nv_bfloat16>(p, st);
-  if (dtype == 1) return launch_snorm<__half>(p, st);
+  if (a->dtype == 0) return launch_snorm<__nv_bfloat16>(p, st);
+  if (a->dtype == 1) return launch_snorm<__half>(p, st);
   return launch_snorm<float>(p, st);
 }

@@ -290,10 +290,18 @@ int tfb_context_attn(const tfb_context_attn_args* a, void* stream);
 // computed from x as it is stored. res / y / x / h: bf16 (dtype 0), fp16 (1) or fp32 (2), rows of C elements, C a multiple
 // of 8 up to 8192, 16-byte rows. w / w2: [C] or null, of the activations' type (w_f32 = 0) or fp32 (1). Tables fp32, each
 // with its own row stride and rows per table row (row r reads table row r / rows_per).
-int tfb_sandwich_norm(const void* res, long ldr, const void* y, long ldy, void* x, void* h, long rows, int C, float eps,
-                      int dtype, int w_f32, const void* w, const void* w2, const float* gate, long ldg, long rpg,
-                      const float* shift, long lds, long rps, const float* scale, long ldc, long rpc, int post,
-                      int tanh_gate, void* stream);
+typedef struct {
+  const void *res, *y;
+  void *x, *h;
+  const void *w, *w2;
+  const float *gate, *shift, *scale;
+  long rows;
+  long ldr, ldy, ldg, rpg, lds, rps, ldc, rpc;  // row strides in elements, rows of the activations per table row
+  int C, dtype, w_f32, post, tanh_gate, reserved0;
+  float eps;
+  int reserved1;
+} tfb_sandwich_norm_args;
+int tfb_sandwich_norm(const tfb_sandwich_norm_args* a, void* stream);
 
 #ifdef __cplusplus
 }

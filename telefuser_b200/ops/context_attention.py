@@ -63,10 +63,13 @@ def _check(q, k, v, what: str) -> None:
     qs, ks = q.shape, k.shape
     if len(qs) != 4 or len(ks) != 4 or ks != v.shape:
         raise ValueError(f"{what}: q [B, Sq, H, D] and k / v of one shape [B, Skv, Hkv, D], got {tuple(qs)}, {tuple(ks)}, {tuple(v.shape)}")
-    if ks[3] != qs[3] or ks[2] < 1 or qs[2] % ks[2]:
-        raise ValueError(f"{what}: heads {qs[2]} x {qs[3]} do not fit key heads {ks[2]} x {ks[3]}")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
-        raise ValueError(f"{what}: q, k and v have one type, got {q.dtype}, {k.dtype}, {v.dtype}")
+    _, _, H, D = qs
+    _, _, Hkv, Dk = ks
+    if Dk != D or Hkv < 1 or H % Hkv:
+        raise ValueError(f"{what}: heads {H} x {D} do not fit key heads {Hkv} x {Dk}")
+    dtype = q.dtype
+    if k.dtype != dtype or v.dtype != dtype:
+        raise ValueError(f"{what}: q, k and v have one type, got {dtype}, {k.dtype}, {v.dtype}")
     native.same_device(q, k, v)
 
 
@@ -91,16 +94,15 @@ def _lengths(lens, n: int, most: int, device, what: str):
     return lens.contiguous() if lens.dtype == torch.int32 else lens.clamp(-1, 2**31 - 1).to(torch.int32)
 
 
-def _operand(t):
-    """-> (tensor, address, batch, token and head strides), with unit channel stride, 16-byte rows and no broadcast dimension:
-    copied only if it is not so already. A dimension of one entry gets stride 0."""
+def _operand(t, rows: int, heads: int, D: int):
+    """t [n, rows, heads, D] -> (tensor, address, batch, token and head strides), with unit channel stride, 16-byte rows and no
+    broadcast dimension: copied only if it is not so already. A dimension of one entry may get any stride."""
     at = t.data_ptr()
-    B, S, H, D = t.shape
-    if t.is_contiguous() and at % 16 == 0 and D % 8 == 0:
-        return t, at, S * H * D, H * D, D
+    if t.is_contiguous() and not at & 15:  # D is a multiple of 8
+        return t, at, rows * heads * D, heads * D, D
     strides = [s if n > 1 else 0 for n, s in zip(t.shape, t.stride())]
-    if at % 16 or (D > 1 and strides[3] != 1) or any(n > 1 and (s <= 0 or s % 8) for n, s in zip(t.shape[:3], strides)):
-        return _operand(t.clone(memory_format=torch.contiguous_format))
+    if at & 15 or strides[3] != 1 or any(n > 1 and (s <= 0 or s % 8) for n, s in zip(t.shape[:3], strides)):
+        return _operand(t.clone(memory_format=torch.contiguous_format), rows, heads, D)
     return t, at, strides[0], strides[1], strides[2]
 
 
@@ -126,27 +128,28 @@ def _launch(q, k, v, kp, vp, kv_lens, cu_kv, key_mask, scale, return_lse):
         with torch.cuda.device(dev):
             return _launch(q, k, v, kp, vp, kv_lens, cu_kv, key_mask, scale, return_lse)
     B, Sq, H, D = q.shape
+    _, Skv, Hkv, _ = k.shape
     P = 0 if kp is None else kp.shape[1]
     if P and B > 1 and Sq > 1 and q.stride(0) != Sq * q.stride(1):
         q = q.contiguous()  # the shared prefix sees the tokens of all samples as one row after the other
-    out = torch.empty((B, Sq, H, D), device=q.device, dtype=q.dtype)
-    lse = torch.empty((B, H, Sq), device=q.device, dtype=torch.float32) if return_lse else None
+    out = torch.empty_like(q) if q.is_contiguous() else torch.empty((B, Sq, H, D), device=q.device, dtype=q.dtype)
+    lse = q.new_empty((B, H, Sq), dtype=torch.float32) if return_lse else None
     if B and Sq and H:
-        q, qp, q_bs, q_ss, q_hs = _operand(q)
-        k, kk, k_bs, k_ss, k_hs = _operand(k)
-        v, vv, v_bs, v_ss, v_hs = _operand(v)
-        pre = (0, 0, 0, 0, 0, 0)
+        q, qp, q_bs, q_ss, q_hs = _operand(q, Sq, H, D)
+        k, kk, k_bs, k_ss, k_hs = _operand(k, Skv, Hkv, D)
+        v, vv, v_bs, v_ss, v_hs = _operand(v, Skv, Hkv, D)
+        a = b = a_ss = a_hs = b_ss = b_hs = 0
         if P:
-            kp, a, _, a_ss, a_hs = _operand(kp)
-            vp, b, _, b_ss, b_hs = _operand(vp)
-            pre = (a, b, a_ss, a_hs, b_ss, b_hs)
-        sizes = (B, Sq, H, k.shape[2], D, k.shape[1], P, int(q.dtype == torch.float16))
+            kp, a, _, a_ss, a_hs = _operand(kp, P, Hkv, D)
+            vp, b, _, b_ss, b_hs = _operand(vp, P, Hkv, D)
+        sizes = (B, Sq, H, Hkv, D, Skv, P, q.dtype == torch.float16)
         need = _work_bytes(dev, cu_kv is not None, key_mask is not None, sizes)
         work = torch.empty(need // 4, device=q.device, dtype=torch.float32) if need else None
         args = _ARGS.pack(
-            qp, kk, vv, pre[0], pre[1], out.data_ptr(), native.ptr(lse) or 0, native.ptr(kv_lens) or 0, native.ptr(cu_kv) or 0,
-            native.ptr(key_mask) or 0, native.ptr(work) or 0, q_bs, q_ss, q_hs, k_bs, k_ss, k_hs, v_bs, v_ss, v_hs, *pre[2:],
-            key_mask.stride(0) if key_mask is not None else 0, *sizes, scale, 0)  # fmt: skip
+            qp, kk, vv, a, b, out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if kv_lens is None else kv_lens.data_ptr(),
+            0 if cu_kv is None else cu_kv.data_ptr(), 0 if key_mask is None else key_mask.data_ptr(),
+            0 if work is None else work.data_ptr(), q_bs, q_ss, q_hs, k_bs, k_ss, k_hs, v_bs, v_ss, v_hs, a_ss, a_hs, b_ss, b_hs,
+            0 if key_mask is None else key_mask.stride(0), *sizes, scale, 0)  # fmt: skip
         native.check(native.load().tfb_context_attn(args, native.stream_ptr()), "tfb_context_attn")
     return (out, lse) if return_lse else out
 

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import math
 import os
+import struct
 
 import torch
 import torch.nn.functional as F
@@ -1134,11 +1135,11 @@ def _row_table(t, B, rows, C):
     """fp32 modulation table of 1, B or `rows` rows of C -> (tensor, address, row stride, rows of the activations per table
     row). Slices of a wider table are used in place (their row stride is kept)."""
     if t is None:
-        return None, None, 0, 1
+        return None, 0, 0, 1
     if t.dtype != torch.float32:
         t = t.float()
     n = t.numel() // C
-    if t.shape[-1] != C or n not in (1, B, rows):
+    if t.shape[-1] != C or (n != 1 and n != B and n != rows):
         raise ValueError(f"a modulation table of shape {tuple(t.shape)} does not fit {B} samples / {rows} rows of {C}")
     at = t.data_ptr()
     if t.is_contiguous() and at % 16 == 0:
@@ -1163,6 +1164,24 @@ def _row_matrix(t, rows, C):
     return t, t.data_ptr(), t.stride(0) if rows > 1 else C
 
 
+def _row_vector(w, as_f32):
+    """-> (tensor, address) of a norm weight, 16-byte aligned."""
+    if w is None:
+        return None, 0
+    if as_f32 and w.dtype != torch.float32:
+        w = w.float()
+    at = w.data_ptr()
+    if not w.is_contiguous() or at % 16:
+        w = w.clone(memory_format=torch.contiguous_format)
+        at = w.data_ptr()
+    return w, at
+
+
+_SNORM_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+# tfb_sandwich_norm_args of csrc/tfb_api.h: 9 pointers, the rows, 8 strides and periods, 6 sizes and flags, eps, one reserved word
+_SNORM_ARGS = struct.Struct("@9Pl8l6ifi")
+
+
 def rmsnorm_gate_residual_modulate(res, y, weight=None, gate=None, next_weight=None, shift=None, scale=None, eps=1e-6,
                                    tanh_gate=True, post_norm=True):  # fmt: skip
     """The end of one sub-layer and the start of the next in one pass -> (x, h):
@@ -1172,59 +1191,51 @@ def rmsnorm_gate_residual_modulate(res, y, weight=None, gate=None, next_weight=N
 
     i.e. `rmsnorm_gate_residual` followed by `rmsnorm_modulate`; h is taken from x as it is stored. With post_norm=False
     y enters without a norm (and without `weight`). res / y: [..., C] bf16, fp16 or fp32 on CUDA with C % 8 == 0 up to 8192, others
-    take the two reference steps; weights [C]; gate / shift / scale: [1 | B, 1, C] or [B, S, C]."""
-    if res.shape != y.shape or res.dtype != y.dtype:
-        raise ValueError(f"residual {res.dtype} {tuple(res.shape)} and branch {y.dtype} {tuple(y.shape)} must match")
-    if not post_norm and weight is not None:
+    take the two reference steps; weights [C]; gate / shift / scale: [1 | B, 1, C] or [B, S, C]. Inference only: no gradient
+    is recorded."""
+    shape, dtype = res.shape, res.dtype
+    if shape != y.shape or dtype != y.dtype:
+        raise ValueError(f"residual {dtype} {tuple(shape)} and branch {y.dtype} {tuple(y.shape)} must match")
+    if weight is not None and not post_norm:
         raise ValueError("post_norm=False takes no weight for the norm of y")
-    C = res.shape[-1]
+    C = shape[-1]
     for w in (weight, next_weight):
-        if w is not None and w.shape != (C,):
+        if w is not None and (w.dim() != 1 or w.numel() != C):
             raise ValueError(f"a norm weight has shape ({C},), got {tuple(w.shape)}")
     native.same_device(res, y, weight, gate, next_weight, shift, scale)
-    if not _native(res) or res.dtype not in _SNORM_TYPES or C % 8 or C > 8192:
+    kind = _SNORM_TYPES.get(dtype)
+    if kind is None or not _native(res) or C % 8 or C > 8192:
         n = _rms(y, weight, eps) if post_norm else y.float()
         if gate is not None:
             n = (gate.float().tanh() if tanh_gate else gate.float()) * n
-        x = (res.float() + n).to(res.dtype)
+        x = (res.float() + n).to(dtype)
         h = _rms(x, next_weight, eps)
         if scale is not None:
             h = h * (1.0 + scale.float())
         if shift is not None:
             h = h + shift.float()
-        return x, h.to(res.dtype)
+        return x, h.to(dtype)
     if res.device.index != torch.cuda.current_device():
         with torch.cuda.device(res.device):
             return rmsnorm_gate_residual_modulate(res, y, weight, gate, next_weight, shift, scale, eps, tanh_gate, post_norm)
-    rows = res.numel() // C if C else 0
-    x = torch.empty(res.shape, device=res.device, dtype=res.dtype)
-    h = torch.empty(res.shape, device=res.device, dtype=res.dtype)
+    x = torch.empty_like(res) if res.is_contiguous() else torch.empty(shape, device=res.device, dtype=dtype)
+    h = torch.empty_like(x)
+    rows = x.numel() // C if C else 0
     if rows == 0:
         return x, h
-    w_f32 = any(w is not None and w.dtype != res.dtype for w in (weight, next_weight))
-
-    def vector(w):
-        if w is None:
-            return None
-        w = (w.float() if w_f32 else w).contiguous()
-        return w if w.data_ptr() % 16 == 0 else w.clone()
-
+    w_f32 = (weight is not None and weight.dtype != dtype) or (next_weight is not None and next_weight.dtype != dtype)
     res, res_at, ldr = _row_matrix(res, rows, C)
     y, y_at, ldy = _row_matrix(y, rows, C)
-    weight, next_weight = vector(weight), vector(next_weight)
-    B = x.shape[0] if x.dim() > 2 else 1
+    weight, w_at = _row_vector(weight, w_f32)
+    next_weight, w2_at = _row_vector(next_weight, w_f32)
+    B = shape[0] if len(shape) > 2 else 1
     gate, gate_at, ldg, rpg = _row_table(gate, B, rows, C)
     shift, shift_at, lds, rps = _row_table(shift, B, rows, C)
     scale, scale_at, ldc, rpc = _row_table(scale, B, rows, C)
-    code = native.load().tfb_sandwich_norm(
-        res_at, ldr, y_at, ldy, x.data_ptr(), h.data_ptr(), rows, C, eps, _SNORM_TYPES[x.dtype], w_f32, native.ptr(weight),
-        native.ptr(next_weight), gate_at, ldg, rpg, shift_at, lds, rps, scale_at, ldc, rpc, post_norm, tanh_gate,
-        native.stream_ptr())  # fmt: skip
-    native.check(code, "tfb_sandwich_norm")
+    args = _SNORM_ARGS.pack(res_at, y_at, x.data_ptr(), h.data_ptr(), w_at, w2_at, gate_at, shift_at, scale_at, rows, ldr, ldy,
+                            ldg, rpg, lds, rps, ldc, rpc, C, kind, w_f32, post_norm, tanh_gate, 0, eps, 0)  # fmt: skip
+    native.check(native.load().tfb_sandwich_norm(args, native.stream_ptr()), "tfb_sandwich_norm")
     return x, h
-
-
-_SNORM_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
 def headnorm_rope_(q, weight_q, cos=None, sin=None, eps=1e-6, k=None, weight_k=None):

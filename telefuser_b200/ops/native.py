@@ -140,9 +140,7 @@ def _declare(lib) -> None:
         "tfb_slab_reduce": [c_void_p, c_int, c_long, c_int, c_long, c_void_p, c_void_p, c_long, c_void_p, c_long, c_int,
                             c_long, c_void_p, c_int, c_long, c_long, c_void_p],
         "tfb_context_attn": [c_char_p, c_void_p],  # tfb_context_attn_args, packed
-        "tfb_sandwich_norm": [c_void_p, c_long, c_void_p, c_long, c_void_p, c_void_p, c_long, c_int, c_float, c_int, c_int,
-                              c_void_p, c_void_p, c_void_p, c_long, c_long, c_void_p, c_long, c_long, c_void_p, c_long,
-                              c_long, c_int, c_int, c_void_p],
+        "tfb_sandwich_norm": [c_char_p, c_void_p],  # tfb_sandwich_norm_args, packed
         "tfb_attn_fwd_peer": [c_void_p, c_long, c_long, c_void_p, c_long, c_long, c_void_p, c_long, c_long, c_void_p,
                               c_int, c_int, c_int, c_long, c_long, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p],
     }  # fmt: skip
@@ -187,7 +185,7 @@ def use_native(t: torch.Tensor) -> bool:
 
 
 def stream_ptr() -> int:
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def check(code: int, what: str) -> None:
