@@ -6,7 +6,7 @@ or group-limited sigmoid-routed experts plus one shared expert. Parameter names 
 checkpoints, so their state dicts load unchanged.
 
 Execution here: one fused-QKV GEMM, `headnorm_rope_` (per-head norm + RoPE on q and k in one launch),
-the tcgen05 attention kernel (head_dim 128), `rmsnorm_modulate` / `rmsnorm_gate_residual` row kernels
+the tcgen05 attention kernel (head_dim 128), `rmsnorm_modulate` / `rmsnorm_gate_residual` (and their fusion) row kernels
 for the sandwich glue, fused gate|up GEMM + SiLU-mul, and for sparse layers the route -> plan ->
 permute -> grouped GEMM -> combine kernel chain of `ops.moe` (optionally expert-parallel). Samples of a
 batch run one after another, each with its text cut to its valid length, which equals the reference's
@@ -263,8 +263,8 @@ class LingBotVideoBlock(nn.Module):
         shift_msa, scale_msa, gate_msa, shift_mlp, scale_mlp, gate_mlp = (mod[:, i : i + 1] for i in range(6))
         h = TF.rmsnorm_modulate(x, self.norm1.weight, shift_msa, scale_msa, self.eps)
         a = self.attn(h, cos, sin, kv_len)
-        x = TF.rmsnorm_gate_residual(x, a, self.norm_post_attn.weight, gate_msa, self.eps)
-        h = TF.rmsnorm_modulate(x, self.norm2.weight, shift_mlp, scale_mlp, self.eps)
+        x, h = TF.rmsnorm_gate_residual_modulate(x, a, self.norm_post_attn.weight, gate_msa, self.norm2.weight, shift_mlp,
+                                                 scale_mlp, self.eps)  # fmt: skip
         m = self.ffn(h, valid) if isinstance(self.ffn, LingBotVideoSparseMoeBlock) else self.ffn(h)
         return TF.rmsnorm_gate_residual(x, m, self.norm_post_ffn.weight, gate_mlp, self.eps)
 

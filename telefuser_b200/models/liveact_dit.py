@@ -21,6 +21,7 @@ from telefuser_b200.core.base_model import BaseModel
 from telefuser_b200.models.wan_dit import (AffineLayerNorm, RMSNormWeight, WanCrossAttention, WanHead, WanImageMLP,
                                            _fuse_linear_weights, rope_angles_1d, sinusoidal_embedding_1d)  # fmt: skip
 from telefuser_b200.ops import functional as TF
+from telefuser_b200.ops.context_attention import cross_attention
 from telefuser_b200.parallel import shard as pshard
 
 
@@ -58,7 +59,7 @@ class SingleStreamAttention(nn.Module):
         first = start_f + (self.sp_rank * n_t if self.sp_flag else 0)
         kv = TF.linear(enc[first : first + n_t].to(xf.dtype), self.kv_linear.weight, self.kv_linear.bias)
         k, v = kv[..., :C].unflatten(-1, (H, D)), kv[..., C:].unflatten(-1, (H, D))
-        o = TF.attention(q, k, v).reshape(B0 * n_t, S, C)
+        o = cross_attention(q, k, v).reshape(B0 * n_t, S, C)
         return TF.linear(o, self.proj.weight, self.proj.bias).reshape(B0, N, C)
 
 

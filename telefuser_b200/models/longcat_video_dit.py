@@ -11,6 +11,7 @@ Role parity: telefuser/models/longcat_video_dit.py:34-1214.
 
 from __future__ import annotations
 
+import itertools
 import math
 
 import torch
@@ -21,6 +22,7 @@ from telefuser_b200.core.base_model import BaseModel
 from telefuser_b200.models.qwen_image_dit import _WeightOnly
 from telefuser_b200.models.wan_dit import AffineLayerNorm, _fuse_linear_weights
 from telefuser_b200.ops import functional as TF
+from telefuser_b200.ops.context_attention import cross_attention, prefix_attention
 from telefuser_b200.parallel import shard as pshard
 
 
@@ -73,9 +75,10 @@ class Attention(nn.Module):
         new_cache = (k.clone(), v.clone()) if return_kv else None
         if kv_cache is not None:
             ck, cv = (c.to(k.device) for c in kv_cache)
-            if ck.shape[0] == 1 and B > 1:
-                ck, cv = ck.expand(B, -1, -1, -1), cv.expand(B, -1, -1, -1)
-            o = TF.attention(q, torch.cat([ck, k], dim=1), torch.cat([cv, v], dim=1))
+            if ck.shape[0] == 1:  # one clean clip for all samples (guidance branches): read in place
+                o = prefix_attention(q, ck, cv, k, v)
+            else:
+                o = TF.attention(q, torch.cat([ck, k], dim=1), torch.cat([cv, v], dim=1))
         elif num_cond_latents and num_cond_latents > 0:
             n_cond = num_cond_latents * (q.shape[1] // shape[0])
             o = torch.cat([TF.attention(q[:, :n_cond], k[:, :n_cond], v[:, :n_cond]), TF.attention(q[:, n_cond:], k, v)], dim=1)
@@ -99,8 +102,9 @@ class MultiHeadCrossAttention(nn.Module):
         self.proj = nn.Linear(dim, dim)
         self.q_norm, self.k_norm = _WeightOnly(self.head_dim), _WeightOnly(self.head_dim)
 
-    def forward(self, x, cond, kv_seqlen: list[int]):
-        """x [B, N, C]; cond [1, sum(kv_seqlen), C] (valid text tokens of all samples in a row)."""
+    def forward(self, x, cond, kv_seqlen):
+        """x [B, N, C]; cond [1, sum of lengths, C], the valid text tokens of all samples in a row; kv_seqlen: the lengths, or
+        their running sum from 0 as an int32 tensor [B + 1] on x's device (see `text_offsets`)."""
         B, N, C = x.shape
         H, D = self.num_heads, self.head_dim
         q = TF.linear(x, self.q_linear.weight, self.q_linear.bias).unflatten(-1, (H, D))
@@ -108,12 +112,13 @@ class MultiHeadCrossAttention(nn.Module):
         k, v = kv[..., :C].unflatten(-1, (H, D)), kv[..., C:].unflatten(-1, (H, D))
         TF.headnorm_rope_(q, self.q_norm.weight, None, None, 1e-6)
         TF.headnorm_rope_(k, self.k_norm.weight, None, None, 1e-6)
-        outs, off = [], 0
-        for b in range(B):  # every sample sees only its own text tokens
-            n = int(kv_seqlen[b])
-            outs.append(TF.attention(q[b : b + 1], k[:, off : off + n], v[:, off : off + n]))
-            off += n
-        return torch.cat(outs).reshape(B, N, C)
+        cu = kv_seqlen if torch.is_tensor(kv_seqlen) else text_offsets(kv_seqlen, x.device)
+        return cross_attention(q, k, v, cu_kv=cu).reshape(B, N, C)  # every sample sees only its own text tokens
+
+
+def text_offsets(lengths, device) -> torch.Tensor:
+    """int32 [B + 1]: where each sample's text tokens begin in the packed row, and the end of the last."""
+    return torch.tensor([0, *itertools.accumulate(int(n) for n in lengths)], dtype=torch.int32, device=device)
 
 
 class FeedForwardSwiGLU(nn.Module):
@@ -307,6 +312,7 @@ class LongCatVideoTransformer3DModel(BaseModel):
             (t,) = pshard.sequence_parallel_shard([t], [1])
             rope, latent_shape = (rc.contiguous(), rs.contiguous()), (x.shape[1], 1, 1)
         offload = getattr(self, "async_offload_manager", None) if self.async_offload_flag else None
+        y_seqlens = text_offsets(y_seqlens, x.device)
         caches = {}
         for i, blk in enumerate(self.blocks):
             if offload is not None:

@@ -24,6 +24,7 @@ from torch import nn
 
 from telefuser_b200.core.base_model import BaseModel
 from telefuser_b200.ops import functional as TF
+from telefuser_b200.ops.context_attention import cross_attention
 
 ADALN_NUM_BASE_PARAMS, ADALN_NUM_CROSS_ATTN_PARAMS = 6, 3
 
@@ -218,6 +219,13 @@ def _masked_attention(q, k, v, mask):
     return (torch.softmax(s, dim=-1) @ v.float().permute(0, 2, 1, 3)).permute(0, 2, 1, 3).to(q.dtype)
 
 
+def _key_masked_attention(q, k, v, visible):
+    """visible: bool [B, S], True where a context token may be seen. A sample without one attends to all of them evenly, as it
+    does under an additive mask of the lowest finite value."""
+    some = visible.any(dim=-1, keepdim=True)
+    return cross_attention(q, torch.where(some[:, :, None, None], k, torch.zeros_like(k)), v, key_mask=visible | ~some)
+
+
 class Attention(nn.Module):
     def __init__(self, query_dim: int, context_dim: int | None = None, heads: int = 8, dim_head: int = 64, norm_eps: float = 1e-6,
                  rope_type: LTXRopeType = LTXRopeType.INTERLEAVED, apply_gated_attention: bool = False) -> None:  # fmt: skip
@@ -248,6 +256,8 @@ class Attention(nn.Module):
             q4, k4, v4 = q.unflatten(-1, (H, D)), k.unflatten(-1, (H, D)), v.unflatten(-1, (H, D))
             if mask is None:
                 out = TF.attention(q4.contiguous(), k4.contiguous(), v4)
+            elif mask.dtype == torch.bool:
+                out = _key_masked_attention(q4, k4, v4, mask)
             else:
                 out = _masked_attention(q4, k4, v4, mask)
             out = out.flatten(-2)
@@ -352,14 +362,14 @@ class BasicAVTransformerBlock(nn.Module):
     def _norm_mod(self, x, scale, shift):
         return TF.rmsnorm_modulate(x, None, shift, scale, self.norm_eps)
 
-    def _text_cross(self, x, args: TransformerArgs, attn: Attention, table, prompt_table):
+    def _text_cross(self, h, args: TransformerArgs, attn: Attention, gate, prompt_table):
+        """h: the normalised (and modulated) stream."""
         if not self.cross_attention_adaln:
-            return attn(TF.rmsnorm_modulate(x, None, None, None, self.norm_eps), context=args.context, mask=args.context_mask)
-        shift_q, scale_q, gate = _ada(table, args.timesteps, slice(6, 9))
+            return attn(h, context=args.context, mask=args.context_mask)
         pt = args.prompt_timestep
-        shift_kv, scale_kv = (prompt_table.float()[None, None] + pt.reshape(x.shape[0], pt.shape[1], 2, -1)).unbind(dim=2)
-        ctx = (args.context.float() * (1 + scale_kv) + shift_kv).to(x.dtype)
-        return (attn(self._norm_mod(x, scale_q, shift_q), context=ctx, mask=args.context_mask).float() * gate).to(x.dtype)
+        shift_kv, scale_kv = (prompt_table.float()[None, None] + pt.reshape(h.shape[0], pt.shape[1], 2, -1)).unbind(dim=2)
+        ctx = (args.context.float() * (1 + scale_kv) + shift_kv).to(h.dtype)
+        return (attn(h, context=ctx, mask=args.context_mask).float() * gate).to(h.dtype)
 
     def _self_branch(self, x, args, attn1, attn2, table, prompt_table, kind, perturbations):
         shift, scale, gate = _ada(table, args.timesteps, slice(0, 3))
@@ -367,8 +377,12 @@ class BasicAVTransformerBlock(nn.Module):
         pmask = perturbations.mask_like(kind, self.idx, x) if (not skip_all and perturbations.any_in_batch(kind, self.idx)) else None
         a = attn1(self._norm_mod(x, scale, shift), pe=args.positional_embeddings, mask=args.self_attention_mask,
                   perturbation_mask=pmask, all_perturbed=skip_all)  # fmt: skip
-        x = TF.gated_residual(x, a, gate)
-        return x + self._text_cross(x, args, attn2, table, prompt_table)
+        shift_q = scale_q = gate_q = None
+        if self.cross_attention_adaln:
+            shift_q, scale_q, gate_q = _ada(table, args.timesteps, slice(6, 9))
+        x, h = TF.rmsnorm_gate_residual_modulate(x, a, None, gate, None, shift_q, scale_q, self.norm_eps, tanh_gate=False,
+                                                 post_norm=False)  # fmt: skip
+        return x + self._text_cross(h, args, attn2, gate_q, prompt_table)
 
     def _av_tables(self, table, args, indices):
         scale, shift = _ada(table[:4], args.cross_scale_shift_timestep, indices)
@@ -499,7 +513,10 @@ class LTXModel(nn.Module):
         ctx = ctx.view(B, -1, ctx.shape[-1])
         cmask = m.context_mask
         if cmask is not None and not torch.is_floating_point(cmask):
-            cmask = (cmask - 1).to(torch.float32).reshape(cmask.shape[0], 1, -1, cmask.shape[-1]) * torch.finfo(torch.float32).max
+            if cmask.numel() == cmask.shape[0] * cmask.shape[-1]:
+                cmask = (cmask > 0).reshape(cmask.shape[0], -1)  # one mark per context token
+            else:
+                cmask = (cmask.to(torch.float32) - 1).reshape(cmask.shape[0], 1, -1, cmask.shape[-1]) * torch.finfo(torch.float32).max
         smask = None
         if m.attention_mask is not None:
             am = m.attention_mask.float()

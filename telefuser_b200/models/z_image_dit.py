@@ -137,8 +137,9 @@ class ZImageTransformerBlock(nn.Module):
             scale_msa = gate_msa = scale_mlp = gate_mlp = None
         tanh = self.modulation
         a = self.attention(TF.rmsnorm_modulate(x, self.attention_norm1.weight, None, scale_msa, self.eps), rope)
-        x = TF.rmsnorm_gate_residual(x, a, self.attention_norm2.weight, gate_msa, self.eps, tanh_gate=tanh)
-        f = self.feed_forward(TF.rmsnorm_modulate(x, self.ffn_norm1.weight, None, scale_mlp, self.eps))
+        x, h = TF.rmsnorm_gate_residual_modulate(x, a, self.attention_norm2.weight, gate_msa, self.ffn_norm1.weight, None,
+                                                 scale_mlp, self.eps, tanh_gate=tanh)  # fmt: skip
+        f = self.feed_forward(h)
         return TF.rmsnorm_gate_residual(x, f, self.ffn_norm2.weight, gate_mlp, self.eps, tanh_gate=tanh)
 
 
