@@ -6,7 +6,8 @@
 // tile; otherwise a tile is 128 tokens of one head. 512 threads:
 //   warp 0   TMA loader                                   warps 4..7    softmax group 0 (query tile 0; TMEM lane == row)
 //   warp 1   tcgen05.mma issuer, TMEM owner               warps 8..11   softmax group 1 (query tile 1)
-//   warp 3   decodes the work items into a ring           warps 12..15  output of finished tiles
+//   warp 3   decodes the work items into a ring, writes   warps 12..15  output of finished tiles
+//            the rows of items without keys
 //   warp 2   tail / mask warp: clears the V rows that nobody may see before the P.V product reads them (a product with
 //            infinities or NaN there would spread through P = 0) and turns the key mask into bit words
 // TMEM (512 columns): S0 | S1 | O0 | O1. P overwrites the first 64 columns of its S tile and enters P.V from TMEM.
@@ -15,9 +16,11 @@
 // and writing a tile is the output warps' business (shared memory, then TMA stores that clip at the tensor's edge) while the
 // softmax groups go on with the next item. The last block of a sample is as narrow as its keys need: 32-column steps in
 // Q.K^T, the exponentials and P.V.
-// The issuer is the warp that everything waits for: a P.V + Q.K^T pair takes the tensor core 1024 clk, and its 16
-// instructions took 1500 clk to issue while descriptors sat in per-lane registers. Its values are warp-uniform by
-// construction (items come through shuffles) and one elected lane issues.
+// The issuer is the warp that everything waits for: a P.V + Q.K^T pair takes the tensor core 1024 clk, and everything else
+// that warp does comes on top, on a scheduler it shares with two softmax warps. So its one wait per tile and block covers
+// P, V, the next K and the accumulator (the tail warp's arrival stands for the loads), its values are warp-uniform, and
+// its view of an item is four integers. (An issuer per tile was slower, 594 for 558 us on two prompts of 512 and 183 tokens:
+// the tensor core takes turns between two warps, and both tiles' chains get longer.)
 //
 // The row maximum that exp2 uses is only raised when it grew by more than 2^8. P is rounded to the inputs' type for the
 // product (at most 2^8, sum in fp32).
@@ -120,7 +123,9 @@ __device__ __forceinline__ int ctx_block_keys(const CtxTcParams& p, int j, int l
   return min(128, j < p.n_prefix ? p.c.P - j * 128 : len - (j - p.n_prefix) * 128);
 }
 
-// The ring of decoded items as one reader warp sees it.
+// The ring of decoded items as one reader warp sees it. All of them have keys: the ring moves on with its slowest reader, and
+// a reader that waits for the last V of an item, which is loaded beside the first K of the next, would hold up the decoder
+// behind a run of items without any.
 struct CtxItems {
   const int4* ring;
   uint64_t *full, *empty;
@@ -139,20 +144,18 @@ struct CtxItems {
     t.j0 = __shfl_sync(0xffffffffu, b.z, 0), t.nb = __shfl_sync(0xffffffffu, b.w, 0);
     return t.b >= 0;
   }
-  // What the issuer needs of the next item with keys: blocks, query tiles, the place of the prefix's last block among them
+  // What the issuer needs of the next item: blocks, query tiles, the place of the prefix's last block among them
   // (or -1), and the columns of that block (low half) and of the item's last. False as above.
   __device__ __forceinline__ bool next_issue(int4& r, const AbortCtx& ctx, int site) {
-    do {
-      const int slot = n % CT_ITEMS;
-      if (!mbar_wait_warp(&full[slot], (n / CT_ITEMS) & 1, ctx, site)) return false;
-      ++n;
-      if (lane_id() == 0) {
-        r = ring[slot * 3 + 2];
-        mbar_arrive(&empty[slot]);
-      }
-      r.x = __shfl_sync(0xffffffffu, r.x, 0), r.y = __shfl_sync(0xffffffffu, r.y, 0);
-      r.z = __shfl_sync(0xffffffffu, r.z, 0), r.w = __shfl_sync(0xffffffffu, r.w, 0);
-    } while (r.x == 0);
+    const int slot = n % CT_ITEMS;
+    if (!mbar_wait_warp(&full[slot], (n / CT_ITEMS) & 1, ctx, site)) return false;
+    ++n;
+    if (lane_id() == 0) {
+      r = ring[slot * 3 + 2];
+      mbar_arrive(&empty[slot]);
+    }
+    r.x = __shfl_sync(0xffffffffu, r.x, 0), r.y = __shfl_sync(0xffffffffu, r.y, 0);
+    r.z = __shfl_sync(0xffffffffu, r.z, 0), r.w = __shfl_sync(0xffffffffu, r.w, 0);
     return r.x > 0;
   }
 };
@@ -272,6 +275,23 @@ __device__ __forceinline__ void ctx_softmax_part(uint32_t tmem_s, uint32_t tmem_
   l += ctx_sum(ps);
 }
 
+// An item without keys: zero rows and -inf, or in split form only the mark that its slot saw nothing. Whole warp.
+__device__ __noinline__ void ctx_no_keys(const CtxTcParams& p, const CtxItem& t) {
+  const int pieces = p.c.D >> 3;  // 16 bytes each
+  for (int x = lane_id(); x < 256 * pieces; x += 32) {
+    const int row = x / pieces, piece = x - row * pieces;
+    const int tok = t.qp * 2 * p.tok + row / p.pack, head = t.hg * p.pack + row % p.pack;
+    if (tok >= p.c.Sq) break;
+    const long token = static_cast<long>(t.b) * p.c.Sq + tok;
+    if (p.c.part_o) {
+      if (piece == 0) p.c.part_lse[(static_cast<long>(p.c.slot0 + t.split) * p.c.B * p.c.Sq + token) * p.c.H + head] = -INFINITY;
+      continue;
+    }
+    reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.c.out) + (token * p.c.H + head) * p.c.D)[piece] = make_uint4(0, 0, 0, 0);
+    if (p.c.lse && piece == 0) p.c.lse[(static_cast<long>(t.b) * p.c.H + head) * p.c.Sq + tok] = -INFINITY;
+  }
+}
+
 template <bool FP16, int DK, bool MASK>
 __global__ void __launch_bounds__(512, 1)
     ctx_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -357,11 +377,8 @@ __global__ void __launch_bounds__(512, 1)
         const int tile_tok = (t.qp * 2 + st) * p.tok;
         const int tok = tile_tok + row_tok, head = t.hg * p.pack + row_head;
         const bool row_ok = tok < p.c.Sq;
-        float2 m_l = make_float2(-INFINITY, 0.f);
-        if (t.nb > 0) {
-          if (!(ok = mbar_wait_warp(&l_full[st], (o_phase >> st) & 1, ctx, 56))) break;
-          m_l = ml[st * 128 + row];
-        }
+        if (!(ok = mbar_wait_warp(&l_full[st], (o_phase >> st) & 1, ctx, 56))) break;
+        const float2 m_l = ml[st * 128 + row];
         const float inv = m_l.y > 0.f ? 1.f / m_l.y : 0.f;
         if (row_ok && (p.c.part_o || p.c.lse)) {
           const float lse2 = m_l.y > 0.f ? m_l.x + log2f(m_l.y) : -INFINITY;
@@ -370,26 +387,22 @@ __global__ void __launch_bounds__(512, 1)
           else
             p.c.lse[(static_cast<long>(t.b) * p.c.H + head) * p.c.Sq + tok] = lse2 * 0.6931471805599453f;
         }
-        if (t.nb > 0) {
-          if (!(ok = mbar_wait_warp(&o_final[st], (o_phase >> st) & 1, ctx, 57))) break;
-          o_phase ^= 1u << st;
-          tc_fence_after();
-        }
+        if (!(ok = mbar_wait_warp(&o_final[st], (o_phase >> st) & 1, ctx, 57))) break;
+        o_phase ^= 1u << st;
+        tc_fence_after();
         const uint32_t tmem_o = tmem_base + lane_addr + 256 + st * 128;
         if (p.c.part_o) {
           const long at = ((static_cast<long>(p.c.slot0 + t.split) * p.c.B + t.b) * p.c.Sq + tok) * p.c.H + head;
-          if (t.nb > 0) {
-            for (int c = 0; c < DK / 16; ++c) {
-              uint32_t o[16];
-              tmem_ld_32x16(tmem_o + c * 16, o);
-              tmem_ld_wait();
+          for (int c = 0; c < DK / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld_32x16(tmem_o + c * 16, o);
+            tmem_ld_wait();
 #pragma unroll
-              for (int e = 0; e < 16; e += 4)
-                if (row_ok && c * 16 + e < p.c.D)
-                  *reinterpret_cast<float4*>(p.c.part_o + at * p.c.D + c * 16 + e) =
-                      make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv,
-                                  __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
-            }
+            for (int e = 0; e < 16; e += 4)
+              if (row_ok && c * 16 + e < p.c.D)
+                *reinterpret_cast<float4*>(p.c.part_o + at * p.c.D + c * 16 + e) =
+                    make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv,
+                                __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
           }
         } else {
           const int first_tok = tile_tok + wq * 32 / p.pack;
@@ -403,13 +416,8 @@ __global__ void __launch_bounds__(512, 1)
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
                 uint32_t o[32];
-                if (t.nb > 0) {
-                  tmem_ld_32x32(tmem_o + x * 64 + c * 32, o);
-                  tmem_ld_wait();
-                } else {
-#pragma unroll
-                  for (int e = 0; e < 32; ++e) o[e] = 0;
-                }
+                tmem_ld_32x32(tmem_o + x * 64 + c * 32, o);
+                tmem_ld_wait();
 #pragma unroll
                 for (int y = 0; y < 4; ++y) {
                   uint4 v;
@@ -431,11 +439,9 @@ __global__ void __launch_bounds__(512, 1)
             }
           }
         }
-        if (t.nb > 0) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&o_empty[st]);
-        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_empty[st]);
       }
     }
     if (lane == 0) tma_store_wait_all();
@@ -596,7 +602,7 @@ __global__ void __launch_bounds__(512, 1)
           }
         };
         uint8_t m[4];
-        if (MASK && t.nb > 0) load_mask(0, m);
+        if (MASK) load_mask(0, m);
         for (int n = 0; n < t.nb; ++n) {
           if (MASK && g == 0 && lane == 0) mbar_arrive(&kv_ready[0]);  // stage 0 has no V and no words
           ++g;  // the stage with this block's V
@@ -645,12 +651,17 @@ __global__ void __launch_bounds__(512, 1)
       int4* ring = reinterpret_cast<int4*>(smem + CT_ITEM_OFF);
       int n = 0, ends_b = -1;
       int2 ends = make_int2(0, 0);
-      for (int i = blockIdx.x;; i += gridDim.x, ++n) {
+      for (int i = blockIdx.x;; i += gridDim.x) {
         const bool end = i >= p.n_items;
-        if (!end)
+        if (!end) {
           t = ctx_item<MASK>(p, i, ends_b, ends);
-        else
+          if (t.nb == 0) {
+            ctx_no_keys(p, t);
+            continue;
+          }
+        } else {
           t.b = -1, t.hg = t.qp = t.split = t.first = t.len = t.j0 = t.nb = 0;
+        }
         const int slot = n % CT_ITEMS;
         if (!mbar_wait_warp(&i_empty[slot], ((n / CT_ITEMS) & 1) ^ 1, ctx, 54)) break;
         if (lane == 0) {
@@ -663,6 +674,7 @@ __global__ void __launch_bounds__(512, 1)
                                          (cut_cols & 0xffff) | last_cols << 16);
           mbar_arrive(&i_full[slot]);
         }
+        ++n;
         if (end) break;
         __syncwarp();
       }
@@ -678,7 +690,6 @@ __global__ void __launch_bounds__(512, 1)
     int ns = 0, no = 0, g = 0;  // score tiles, items with keys and key blocks seen so far
     bool ok = true;
     while (ok && items.next(t, ctx, 58)) {
-      if (t.nb == 0) continue;
       if (st && !t.two(p)) {
         g += t.nb;
         continue;

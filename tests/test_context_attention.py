@@ -263,6 +263,25 @@ def test_peaked_scores_and_scale(lib, Sq, dtype):
     check(*CA.cross_attention(q, k, v, scale=0.2, return_lse=True), exact(q, [(k[b], v[b]) for b in range(2)], 0.2), dtype)
 
 
+
+@gpu
+@pytest.mark.parametrize("layout", ["padded", "packed", "masked"])
+def test_long_runs_of_tiles_without_keys(lib, layout):
+    """Samples without states among others, each of them several tiles per SM, with one and with three blocks of keys."""
+    B, Sq, H, D = 4, 24001, 8, 64
+    lens = [300, 0, 0, 90]
+    q, k, v = make(B, Sq, H, H, D, 300, BF, "cuda", seed=11)
+    visible = torch.arange(300, device="cuda")[None] < torch.tensor(lens, device="cuda")[:, None]
+    if layout == "packed":
+        o, lse = CA.cross_attention(q, k[visible], v[visible], cu_kv=[0, 300, 300, 300, 390], return_lse=True)
+    elif layout == "padded":
+        o, lse = CA.cross_attention(q, k, v, kv_lens=lens, return_lse=True)
+    else:
+        o, lse = CA.cross_attention(q, k, v, key_mask=visible, return_lse=True)
+    check(o, lse, exact(q, pick(k, v, visible)), BF)
+    assert (o[1:3] == 0).all() and (lse[1:3] == float("-inf")).all()
+
+
 @gpu
 @pytest.mark.parametrize("Sq", [2, 130])
 def test_device_lengths_out_of_range_are_clamped(lib, Sq):
