@@ -4,8 +4,9 @@
 // One CTA of four warps owns the <= 32 query rows of one (sample, key head) - tokens x grouped heads - and one slice of the
 // keys. Its warps work for themselves, 16 keys at a time: a warp has a ring of TMA boxes in shared memory (K and V of 16 keys
 // each), its own running maximum, sum and fp32 accumulator, and refills a slot as soon as it has read it; the four results
-// are joined once at the end. So bytes in flight cost no registers: two CTAs per SM hold about 180 KB of the stream, and no
-// warp waits for another. The products run on mma.sync m16n8k16, fed by ldmatrix: with so few rows the tensor work is a
+// are joined once at the end. So bytes in flight cost no registers: two CTAs per SM hold 192 KB of the stream, and no
+// warp waits for another. (Three with two thirds of the ring each: 187 for 154 us on 64 streams x 8 key heads x 4096 keys, whose 512
+// CTAs then leave a second wave of 68.) The products run on mma.sync m16n8k16, fed by ldmatrix: with so few rows the tensor work is a
 // fraction of what the loads take.
 // Keys that the length or the mask hides: their scores are replaced by -inf and their V fragments by zeros, so infinities
 // and NaN there never meet a product.
@@ -56,18 +57,19 @@ __device__ __forceinline__ uint32_t box_at(int row, int piece) {
 template <int DK, int MT>
 struct CtxRowsCfg {
   static constexpr int CHUNK = 2 * 16 * DK * 2;             // K and V of 16 keys
-  static constexpr int STAGES = DK == 128 ? 3 : 6;          // per warp: 24 KB in flight
-  static constexpr int RING = CR_WARPS * STAGES * CHUNK;    // 96 KB; the join at the end lies over it
+  static constexpr int CTAS = 2;                            // per SM
+  static constexpr int STAGES = 24576 / CHUNK;              // per warp
+  static constexpr int RING = CR_WARPS * STAGES * CHUNK;    // the join at the end lies over it
   static constexpr int Q_OFF = RING;                        // MT x 16 rows as boxes
   static constexpr int ML_OFF = Q_OFF + MT * 16 * DK * 2;   // [warps][MT * 16] of (maximum, sum)
   static constexpr int BAR_OFF = ML_OFF + CR_WARPS * MT * 16 * 8;
   static constexpr int SMEM = BAR_OFF + CR_WARPS * STAGES * 8 + 16 + 1024;
   static_assert(CR_WARPS * MT * 16 * DK * 4 <= RING, "the join fits over the ring");
-  static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs per SM");
+  static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "CTAs per SM");
 };
 
 template <bool FP16, int DK, int MT>
-__global__ void __launch_bounds__(CR_WARPS * 32, 2)
+__global__ void __launch_bounds__(CR_WARPS * 32, CtxRowsCfg<DK, MT>::CTAS)
     ctx_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                     const __grid_constant__ CUtensorMap tmKp, const __grid_constant__ CUtensorMap tmVp,
                     const __grid_constant__ CtxRowsParams rp) {

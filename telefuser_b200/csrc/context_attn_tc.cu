@@ -761,6 +761,8 @@ int launch_ctx_tc(const CtxParams& c, int fp16, cudaStream_t st) {
   p.bmul = packed ? 0 : 1;
   const long items = ctx_tc_items(c.B, c.Sq, c.H, c.Hkv) * c.ns;
   if (items > 0x3fffffffL) return TFB_ERR_TOO_LARGE;
+  // An item takes about 2 us per 128 keys, and the output warps wait for all of it: well inside their bounded wait (0.8 s).
+  if ((static_cast<long>(c.Skv) + c.P) / c.ns > (1L << 24)) return TFB_ERR_TOO_LARGE;
   p.n_items = static_cast<int>(items);
   CUtensorMap tm[6];
   const int kb = packed ? 1 : c.B;
