@@ -5,8 +5,10 @@
 // head) in shared memory, and every warp takes tiles of 16 query rows - (token, grouped head) pairs, any group size - straight
 // from global memory into mma.sync fragments, softmax in registers, results straight to global memory, the next tile's
 // queries already on their way. 16 to 20 warps per SM hold 64 KB and more of loads in flight. (The tensor-memory kernel hands every
-// tile through five warps and their barriers, which costs it about 10,000 clk per 256 rows whatever the keys: 258 us against
-// this kernel's figure for 21 frames of 1560 tokens x 40 heads against 32 keys.)
+// tile through five warps and their barriers, about 10,000 clk per 256 rows whatever the keys: 258 us against 138 here for 21
+// frames of 1560 tokens x 40 heads against 32 keys, 4.9 TB/s, three quarters of what a copy reaches. At its upper end the two meet: 20000 tokens
+// x 32 heads take 108 us with 64 keys here, 111 with 65 there.) What bounds it then is L1: every query and output byte
+// passes it in 16-byte pieces of eight rows at a time (79 % busy), half of all issue slots are taken.
 // Coalescing comes from permuting indexes: a lane loads and stores whole 16-byte pieces of a row, and the copies of K and V
 // in shared memory have their channels reordered to match what the fragments then hold:
 //   Q.K^T  lane (n, c) = (lane / 4, lane % 4) holds channels 32 i + 8 c .. + 7 of row n; it feeds pair w (channels 2 w, 2 w + 1

@@ -5,6 +5,7 @@
     python -m telefuser_b200.ops.kernel_bench elementwise --rows 75600 --dim 5120
     python -m telefuser_b200.ops.kernel_bench moe   --tokens 16384
     python -m telefuser_b200.ops.kernel_bench vae   --frames 17 --height 480 --width 832
+    python -m telefuser_b200.ops.kernel_bench context --case clip_to_prompts
     python -m telefuser_b200.ops.kernel_bench all
 
 Timing: CUDA events on the launching stream, `--warmup` untimed launches, then `--iters` timed ones;
@@ -244,9 +245,68 @@ def bench_vae(t: Timer, frames: int, height: int, width: int, compare: bool) -> 
                frames=T, height=height, width=width)  # fmt: skip
 
 
+def bench_context(t: Timer, case: str | None) -> None:
+    """Conditioning: attention to states of another length, a prefix shared by the batch, the sandwich norm between two
+    sub-layers. `case` picks one."""
+    from telefuser_b200.ops import context_attention as CA
+
+    def normal(*shape, dtype=torch.bfloat16):
+        return torch.randn(*shape, device="cuda").to(dtype)
+
+    def cross(B, Sq, H, Hkv, D, lens, dtype=torch.bfloat16, packed=False, masked=False):
+        q, most = normal(B, Sq, H, D, dtype=dtype), max(lens)
+        kw = {}
+        if packed:
+            k, v = normal(sum(lens), Hkv, D, dtype=dtype), normal(sum(lens), Hkv, D, dtype=dtype)
+            kw["cu_kv"] = torch.tensor([sum(lens[:i]) for i in range(B + 1)], dtype=torch.int32, device="cuda")
+        else:
+            k, v = normal(B, most, Hkv, D, dtype=dtype), normal(B, most, Hkv, D, dtype=dtype)
+            n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+            if masked:  # padding on the left
+                kw["key_mask"] = torch.arange(most, device="cuda")[None] >= most - n[:, None]
+            elif min(lens) < most:
+                kw["kv_lens"] = n
+        ms = t(lambda: CA.cross_attention(q, k, v, **kw))
+        return ms, 4 * Sq * H * D * sum(lens), 4 * q.numel() + 4 * sum(lens) * Hkv * D, dict(batch=B, tokens=Sq, heads=H, key_heads=Hkv, dim=D, keys=most)
+
+    def prefix(B, Sq, H, Hkv, D, P, lens):
+        q, k, v = normal(B, Sq, H, D), normal(B, max(lens), Hkv, D), normal(B, max(lens), Hkv, D)
+        kp, vp = normal(1, P, Hkv, D), normal(1, P, Hkv, D)
+        n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        ms = t(lambda: CA.prefix_attention(q, kp, vp, k, v, kv_lens=n))
+        return (ms, 4 * Sq * H * D * (B * P + sum(lens)), 4 * q.numel() + 4 * (P + sum(lens)) * Hkv * D,
+                dict(batch=B, tokens=Sq, heads=H, key_heads=Hkv, dim=D, prefix=P, keys=max(lens)))  # fmt: skip
+
+    def norm(B, S, C, dtype=torch.bfloat16, token=False):
+        res, y = normal(B, S, C, dtype=dtype), normal(B, S, C, dtype=dtype)
+        w = None if token else normal(C, dtype=dtype)
+        gate, shift, scale = (torch.randn(B, S if token else 1, C, device="cuda") for _ in range(3))
+        next_w = normal(C, dtype=dtype)
+        ms = t(lambda: TF.rmsnorm_gate_residual_modulate(res, y, w, gate, next_w, shift, scale, tanh_gate=not token, post_norm=not token))
+        return ms, 0, 8 * res.numel() + 3 * 4 * gate.numel(), dict(batch=B, rows=S, dim=C, tables="token" if token else "sample")
+
+    cases = {
+        "one_token": lambda: cross(8, 1, 16, 16, 64, [220, 1, 366, 147, 512, 293, 74, 439], torch.float16),
+        "frames_to_audio": lambda: cross(21, 1560, 40, 40, 128, [32] * 21),
+        "clip_to_prompts": lambda: cross(2, 37440, 32, 32, 128, [512, 183], packed=True),
+        "masked_prompts": lambda: cross(2, 6143, 32, 32, 64, [1024, 77], torch.float16, masked=True),
+        "few_to_long": lambda: cross(1, 5, 32, 8, 128, [131072]),
+        "clip_continuation": lambda: prefix(2, 3120, 32, 32, 128, 9360, [3120, 3120]),
+        "many_streams": lambda: prefix(64, 1, 32, 8, 128, 16384, [15 * i for i in range(64)]),
+        "norm_image": lambda: norm(2, 4224, 3840),
+        "norm_clip": lambda: norm(1, 37441, 2048),
+        "norm_token_tables": lambda: norm(2, 3001, 4096, torch.float16, token=True),
+    }
+    for name, fn in cases.items():
+        if case in (None, name):
+            ms, flops, nbytes, cfg = fn()
+            report(f"context: {name}", ms, flops, nbytes, **cfg)
+
+
 def main() -> None:
     ap = argparse.ArgumentParser()
-    ap.add_argument("what", choices=["attn", "gemm", "elementwise", "moe", "vae", "all"])
+    ap.add_argument("what", choices=["attn", "gemm", "elementwise", "moe", "vae", "context", "all"])
+    ap.add_argument("--case", default=None, help="context: one case by name")
     ap.add_argument("--frames", type=int, default=17)
     ap.add_argument("--height", type=int, default=480)
     ap.add_argument("--width", type=int, default=832)
@@ -278,6 +338,8 @@ def main() -> None:
         bench_elementwise(t, a.rows, a.dim)
     if a.what in ("moe", "all"):
         bench_moe(t, a.tokens, cmp_)
+    if a.what in ("context", "all"):
+        bench_context(t, a.case)
     if a.what == "vae":
         bench_vae(t, a.frames, a.height, a.width, cmp_)
 
