@@ -1131,16 +1131,24 @@ def rmsnorm_gate_residual(res, y, weight=None, gate=None, eps=1e-6, tanh_gate=Tr
     return out.view(res.shape)
 
 
-def _row_table(t, B, rows, C):
-    """fp32 modulation table of 1, B or `rows` rows of C -> (tensor, address, row stride, rows of the activations per table
+def _check_table(t, shape) -> None:
+    """A modulation table has one row of C, one per sample ([B, 1, C]) or one per row of the activations (their shape):
+    rows that would have to repeat in any other way ([1, S, C] under several samples) are refused, not guessed."""
+    ts = t.shape
+    if ts == shape or (ts[-1:] == shape[-1:] and t.numel() == shape[-1]):
+        return
+    if len(ts) != len(shape) or len(ts) < 3 or ts[0] != shape[0] or ts[-1] != shape[-1] or t.numel() != ts[0] * ts[-1]:
+        raise ValueError(f"a modulation table of shape {tuple(ts)} does not fit activations of shape {tuple(shape)}")
+
+
+def _row_table(t, rows, C):
+    """fp32 modulation table that `_check_table` accepted -> (tensor, address, row stride, rows of the activations per table
     row). Slices of a wider table are used in place (their row stride is kept)."""
     if t is None:
         return None, 0, 0, 1
     if t.dtype != torch.float32:
         t = t.float()
     n = t.numel() // C
-    if t.shape[-1] != C or (n != 1 and n != B and n != rows):
-        raise ValueError(f"a modulation table of shape {tuple(t.shape)} does not fit {B} samples / {rows} rows of {C}")
     at = t.data_ptr()
     if t.is_contiguous() and at % 16 == 0:
         return t, at, C, rows // n
@@ -1191,8 +1199,8 @@ def rmsnorm_gate_residual_modulate(res, y, weight=None, gate=None, next_weight=N
 
     i.e. `rmsnorm_gate_residual` followed by `rmsnorm_modulate`; h is taken from x as it is stored. With post_norm=False
     y enters without a norm (and without `weight`). res / y: [..., C] bf16, fp16 or fp32 on CUDA with C % 8 == 0 up to 8192, others
-    take the two reference steps; weights [C]; gate / shift / scale: [1 | B, 1, C] or [B, S, C]. Inference only: no gradient
-    is recorded."""
+    take the two reference steps; weights [C]; gate / shift / scale: C values for all, [B, 1, C] or [B, S, C]. Inference only: no
+    gradient is recorded."""
     shape, dtype = res.shape, res.dtype
     if shape != y.shape or dtype != y.dtype:
         raise ValueError(f"residual {dtype} {tuple(shape)} and branch {y.dtype} {tuple(y.shape)} must match")
@@ -1202,6 +1210,9 @@ def rmsnorm_gate_residual_modulate(res, y, weight=None, gate=None, next_weight=N
     for w in (weight, next_weight):
         if w is not None and (w.dim() != 1 or w.numel() != C):
             raise ValueError(f"a norm weight has shape ({C},), got {tuple(w.shape)}")
+    for t in (gate, shift, scale):
+        if t is not None:
+            _check_table(t, shape)
     native.same_device(res, y, weight, gate, next_weight, shift, scale)
     kind = _SNORM_TYPES.get(dtype)
     if kind is None or not _native(res) or C % 8 or C > 8192:
@@ -1228,10 +1239,9 @@ def rmsnorm_gate_residual_modulate(res, y, weight=None, gate=None, next_weight=N
     y, y_at, ldy = _row_matrix(y, rows, C)
     weight, w_at = _row_vector(weight, w_f32)
     next_weight, w2_at = _row_vector(next_weight, w_f32)
-    B = shape[0] if len(shape) > 2 else 1
-    gate, gate_at, ldg, rpg = _row_table(gate, B, rows, C)
-    shift, shift_at, lds, rps = _row_table(shift, B, rows, C)
-    scale, scale_at, ldc, rpc = _row_table(scale, B, rows, C)
+    gate, gate_at, ldg, rpg = _row_table(gate, rows, C)
+    shift, shift_at, lds, rps = _row_table(shift, rows, C)
+    scale, scale_at, ldc, rpc = _row_table(scale, rows, C)
     args = _SNORM_ARGS.pack(res_at, y_at, x.data_ptr(), h.data_ptr(), w_at, w2_at, gate_at, shift_at, scale_at, rows, ldr, ldy,
                             ldg, rpg, lds, rps, ldc, rpc, C, kind, w_f32, post_norm, tanh_gate, 0, eps, 0)  # fmt: skip
     native.check(native.load().tfb_sandwich_norm(args, native.stream_ptr()), "tfb_sandwich_norm")

@@ -66,6 +66,23 @@ def test_refusals(change):
         TF.rmsnorm_gate_residual_modulate(**a)
 
 
+@pytest.mark.parametrize("shape", [(1, 5, 24), (1, 2, 24), (2, 24), (5, 24), (5, 1, 24), (2, 2, 24), (2, 1, 16), (48,)])
+@pytest.mark.parametrize("which", ["gate", "shift", "scale"])
+@pytest.mark.parametrize("S", [5, 2])
+def test_tables_that_repeat_in_no_documented_way_are_refused(shape, which, S):
+    a = inputs(2, S, 24, torch.float32, "cpu")
+    if shape == (2, S, 24):
+        return
+    with pytest.raises(ValueError):
+        TF.rmsnorm_gate_residual_modulate(**(a | {which: torch.zeros(shape)}))
+
+
+@pytest.mark.parametrize("shape", [(24,), (1, 24), (1, 1, 24), (2, 1, 24), (2, 2, 24)])
+def test_tables_that_fit(shape):
+    a = inputs(2, 2, 24, torch.float32, "cpu") | dict(scale=torch.randn(shape))
+    check(*TF.rmsnorm_gate_residual_modulate(**a), a)
+
+
 # ---- GPU --------------------------------------------------------------------------------------------------------------
 gpu = pytest.mark.gpu
 
