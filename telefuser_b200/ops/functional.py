@@ -1131,26 +1131,27 @@ def rmsnorm_gate_residual(res, y, weight=None, gate=None, eps=1e-6, tanh_gate=Tr
     return out.view(res.shape)
 
 
-def _check_table(t, shape) -> None:
-    """A modulation table has one row of C, one per sample ([B, 1, C]) or one per row of the activations (their shape):
-    rows that would have to repeat in any other way ([1, S, C] under several samples) are refused, not guessed."""
-    ts = t.shape
-    if ts == shape or (ts[-1:] == shape[-1:] and t.numel() == shape[-1]):
-        return
-    if len(ts) != len(shape) or len(ts) < 3 or ts[0] != shape[0] or ts[-1] != shape[-1] or t.numel() != ts[0] * ts[-1]:
+def _table_rows(t, shape, C) -> int:
+    """Rows of a modulation table: one, one per sample ([B, 1, C]) or one per row of the activations (their shape). Rows that
+    would have to repeat in any other way ([1, S, C] under several samples) are refused, not guessed."""
+    ts, n = t.shape, t.numel()
+    if not ts or ts[-1] != C or not (
+        n == C or ts == shape or (len(ts) == len(shape) > 2 and ts[0] == shape[0] and n == ts[0] * C)
+    ):
         raise ValueError(f"a modulation table of shape {tuple(ts)} does not fit activations of shape {tuple(shape)}")
+    return n // C if C else 0
 
 
-def _row_table(t, rows, C):
-    """fp32 modulation table that `_check_table` accepted -> (tensor, address, row stride, rows of the activations per table
-    row). Slices of a wider table are used in place (their row stride is kept)."""
+def _row_table(t, shape, rows, C):
+    """fp32 modulation table -> (tensor, address, row stride, rows of the activations per table row). Slices of a wider table
+    are used in place (their row stride is kept)."""
     if t is None:
         return None, 0, 0, 1
+    n = _table_rows(t, shape, C)
     if t.dtype != torch.float32:
         t = t.float()
-    n = t.numel() // C
     at = t.data_ptr()
-    if t.is_contiguous() and at % 16 == 0:
+    if not at % 16 and t.is_contiguous():
         return t, at, C, rows // n
     lead = [(m, st) for m, st in zip(t.shape[:-1], t.stride()[:-1]) if m > 1]
     if len(lead) > 1 and all(lead[i][1] == lead[i + 1][0] * lead[i + 1][1] for i in range(len(lead) - 1)):
@@ -1210,12 +1211,12 @@ def rmsnorm_gate_residual_modulate(res, y, weight=None, gate=None, next_weight=N
     for w in (weight, next_weight):
         if w is not None and (w.dim() != 1 or w.numel() != C):
             raise ValueError(f"a norm weight has shape ({C},), got {tuple(w.shape)}")
-    for t in (gate, shift, scale):
-        if t is not None:
-            _check_table(t, shape)
     native.same_device(res, y, weight, gate, next_weight, shift, scale)
     kind = _SNORM_TYPES.get(dtype)
     if kind is None or not _native(res) or C % 8 or C > 8192:
+        for t in (gate, shift, scale):
+            if t is not None:
+                _table_rows(t, shape, C)
         n = _rms(y, weight, eps) if post_norm else y.float()
         if gate is not None:
             n = (gate.float().tanh() if tanh_gate else gate.float()) * n
@@ -1239,9 +1240,9 @@ def rmsnorm_gate_residual_modulate(res, y, weight=None, gate=None, next_weight=N
     y, y_at, ldy = _row_matrix(y, rows, C)
     weight, w_at = _row_vector(weight, w_f32)
     next_weight, w2_at = _row_vector(next_weight, w_f32)
-    gate, gate_at, ldg, rpg = _row_table(gate, rows, C)
-    shift, shift_at, lds, rps = _row_table(shift, rows, C)
-    scale, scale_at, ldc, rpc = _row_table(scale, rows, C)
+    gate, gate_at, ldg, rpg = _row_table(gate, shape, rows, C)
+    shift, shift_at, lds, rps = _row_table(shift, shape, rows, C)
+    scale, scale_at, ldc, rpc = _row_table(scale, shape, rows, C)
     args = _SNORM_ARGS.pack(res_at, y_at, x.data_ptr(), h.data_ptr(), w_at, w2_at, gate_at, shift_at, scale_at, rows, ldr, ldy,
                             ldg, rpg, lds, rps, ldc, rpc, C, kind, w_f32, post_norm, tanh_gate, 0, eps, 0)  # fmt: skip
     native.check(native.load().tfb_sandwich_norm(args, native.stream_ptr()), "tfb_sandwich_norm")

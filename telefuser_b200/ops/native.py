@@ -250,6 +250,7 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def same_device(ref: torch.Tensor, *others: torch.Tensor | None) -> None:
     """Raises when an operand lives on another device than `ref` (a module moved after its tensors were tagged)."""
+    device = ref.device
     for t in others:
-        if t is not None and t.device != ref.device:
-            raise NativeLibraryError(f"operand on {t.device}, expected {ref.device} (shape {tuple(t.shape)})")
+        if t is not None and t.device != device:
+            raise NativeLibraryError(f"operand on {t.device}, expected {device} (shape {tuple(t.shape)})")
