@@ -518,7 +518,6 @@ __global__ void __launch_bounds__(512, 1)
       int g = 0;
       uint32_t q_phase = 0, p_phase = 0;  // bit per query tile
       bool ok = true;
-      
       // one lane: Q.K^T of `cols` columns of ring block gg into S of query tile st; `last`: the item's last block
       auto issue_qk = [&](int st, int gg, int cols, bool last) {
         const uint32_t idesc = make_idesc(128, 0, FMT, FMT, 0, 0) | (static_cast<uint32_t>(cols >> 3) << 17);
