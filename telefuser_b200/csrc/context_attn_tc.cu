@@ -608,7 +608,10 @@ __global__ void __launch_bounds__(512, 1)
         uint8_t m[4];
         if (MASK) load_mask(0, m);
         for (int n = 0; n < t.nb; ++n) {
-          if (MASK && g == 0 && lane == 0) mbar_arrive(&kv_ready[0]);  // stage 0 has no V and no words
+          // Stage 0 has no V and no words, but its load is waited for all the same: nothing orders it before that of stage 1, and
+          // until it is complete the parity that stage 2 waits for in this slot is that of a barrier that was never used.
+          if (g == 0 && !(ok = mbar_wait_warp(&kv_full[0], 0, ctx, 51))) break;
+          if (MASK && g == 0 && lane == 0) mbar_arrive(&kv_ready[0]);
           ++g;  // the stage with this block's V
           const int slot = g & 1;
           const int keys = ctx_block_keys(p, t.j0 + n, t.len);

@@ -339,3 +339,23 @@ def test_same_bits_again_on_another_stream_and_replayed(lib, Sq, Skv):
     torch.cuda.synchronize()
     now = [CA.cross_attention(q, k, v, kv_lens=lens), CA.prefix_attention(q, kp, vp, k, v, kv_lens=lens)]
     assert all(torch.equal(a, b) for a, b in zip(outs, now))
+
+
+@gpu
+@pytest.mark.parametrize("fp16", [False, True])
+def test_first_block_arrives_last(lib, fp16):
+    """The tile kernel's first K tile comes from memory while the second block and the first V tile are in L2, so the load of
+    its first stage is the slowest; the keys end inside the second block, behind NaN."""
+    dtype = FP if fp16 else BF
+    B, Sq, H, D, Skv, n = 148, 40, 1, 128, 256, 177
+    q, k, v = make(B, Sq, H, H, D, Skv, dtype, "cuda", seed=12)
+    visible = (torch.arange(Skv, device="cuda") < n).expand(B, -1)
+    k, v = poison(k, visible), poison(v, visible)
+    lens = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    want = exact(q, pick(k, v, visible))
+    flush = torch.empty(64 << 20, device="cuda", dtype=torch.float32)  # twice the L2 cache
+    for _ in range(20):
+        flush.fill_(1.0)
+        (k[:, 128:].isnan().sum() + v[:, :128].isnan().sum() + q.isnan().sum())
+        o, lse = CA.cross_attention(q, k, v, kv_lens=lens, return_lse=True)
+        check(o, lse, want, dtype)
