@@ -17,7 +17,7 @@ struct CtxParams {
   void* out;        // [B, Sq, H, D] contiguous
   float* lse;       // [B, H, Sq] or null
   float* part_o;    // non-null: results go to slots [slot][B * Sq][H][D] (each slot normalised by its own sum) ...
-  float* part_lse;  // ... with base-2 log-sum-exps [slot][B * Sq][H]; -inf marks a slot that saw no key (its part_o is not written)
+  float* part_lse;  // ... with base-2 log-sum-exps [slot][B * Sq][H]; a slot that saw no key holds -inf and zeros
   const int* kv_lens;
   const int* cu_kv;
   const uint8_t* key_mask;
@@ -40,6 +40,17 @@ __device__ __forceinline__ void ctx_sample_range(const CtxParams& p, int b, int&
     len = p.kv_lens ? min(max(__ldg(p.kv_lens + b), 0), p.Skv) : p.Skv;
   }
 }
+
+// What exp2 takes off the scores of a row with the largest score m: m itself, but nothing where m is infinite. Without a key
+// (m = -inf) every weight is then 0; with a score of +inf that one weighs +inf, and so does the sum, while a sum with a NaN
+// score in it is NaN (the maximum passes NaN over). So the sum says all there is to know: 0 where nothing was seen, +inf or
+// NaN where the log-sum-exp is the same and the row NaN, as in a plain evaluation.
+__device__ __forceinline__ float ctx_exp_base(float m) { return fabsf(m) == INFINITY ? 0.f : m; }
+// Factor on what was summed under the maximum m once it is m_new; 1 for an infinity that stays.
+__device__ __forceinline__ float ctx_rescale(float m, float m_new) { return m == m_new ? 1.f : fast_exp2(m - m_new); }
+// 1 / sum, 0 for a row that saw nothing. NaN and +inf (whose row is made of infinities and NaN) lead to NaN.
+__device__ __forceinline__ float ctx_inverse(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }
+__device__ __forceinline__ float ctx_lse2(float m, float sum) { return sum == 0.f ? -INFINITY : m + log2f(sum); }
 
 template <bool FP16>
 __device__ __forceinline__ uint32_t ctx_pack2(float lo, float hi) {

@@ -196,13 +196,13 @@ __global__ void __launch_bounds__(CR_WARPS * 32, CtxRowsCfg<DK, MT>::CTAS)
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         const float m_new = fmaxf(m[mt][r], mx);
         if (__any_sync(0xffffffffu, m_new > m[mt][r])) {
-          const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m[mt][r] - m_new);
+          const float alpha = ctx_rescale(m[mt][r], m_new);
           l[mt][r] *= alpha;
 #pragma unroll
           for (int t = 0; t < DK / 8; ++t) o[mt][t][r * 2] *= alpha, o[mt][t][r * 2 + 1] *= alpha;
           m[mt][r] = m_new;
         }
-        const float base = m[mt][r] == -INFINITY ? 0.f : m[mt][r];
+        const float base = ctx_exp_base(m[mt][r]);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const float p0 = fast_exp2(s[mt][t][r * 2] - base), p1 = fast_exp2(s[mt][t][r * 2 + 1] - base);
@@ -256,26 +256,24 @@ __global__ void __launch_bounds__(CR_WARPS * 32, CtxRowsCfg<DK, MT>::CTAS)
     float mm = s_ml[row].x;
 #pragma unroll
     for (int w = 1; w < CR_WARPS; ++w) mm = fmaxf(mm, s_ml[w * ROWS + row].x);
-    const float base = mm == -INFINITY ? 0.f : mm;
     float sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < CR_WARPS; ++w) {
       const float2 ml = s_ml[w * ROWS + row];
-      const float f = fast_exp2(ml.x - base);
+      const float f = ctx_rescale(ml.x, mm);
       sum += f * ml.y;
       const float4 t = *reinterpret_cast<const float4*>(s_o + (w * ROWS + row) * DK + d);
       acc.x += f * t.x, acc.y += f * t.y, acc.z += f * t.z, acc.w += f * t.w;
     }
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    const float inv = ctx_inverse(sum);
     const long token = static_cast<long>(b) * p.Sq + row / G;
     const int head = hk * G + row % G;
-    const float lse2 = mm == -INFINITY ? -INFINITY : mm + log2f(sum);
+    const float lse2 = ctx_lse2(mm, sum);
     if (p.part_o) {
       const long at = (static_cast<long>(p.slot0 + split) * p.B * p.Sq + token) * p.H + head;
       if (d == 0) p.part_lse[at] = lse2;
-      if (mm != -INFINITY)
-        *reinterpret_cast<float4*>(p.part_o + at * p.D + d) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+      *reinterpret_cast<float4*>(p.part_o + at * p.D + d) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
     } else {
       uint16_t* op = static_cast<uint16_t*>(p.out) + (token * p.H + head) * p.D + d;
       *reinterpret_cast<uint2*>(op) = make_uint2(ctx_pack2<FP16>(acc.x * inv, acc.y * inv), ctx_pack2<FP16>(acc.z * inv, acc.w * inv));
@@ -297,15 +295,15 @@ __global__ void __launch_bounds__(128) ctx_join_kernel(const CtxParams p) {
   float mm = -INFINITY;
   for (int s = lane; s < p.ns; s += 32) mm = fmaxf(mm, p.part_lse[s * rows + row]);
   mm = warp_max(mm);
-  const float base = mm == -INFINITY ? 0.f : mm;
+  const float base = ctx_exp_base(mm);
   float sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   const int d = lane * 4;
 #pragma unroll 4
   for (int s = warp; s < p.ns; s += 4) {
-    const float f = fast_exp2(p.part_lse[s * rows + row] - base);  // 0 for a slot that saw no key: its part_o holds nothing
+    const float f = fast_exp2(p.part_lse[s * rows + row] - base);  // 0 for a slot that saw no key, NaN or +inf for what came so
     float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (d < p.D && f > 0.f) t = *reinterpret_cast<const float4*>(p.part_o + (s * rows + row) * p.D + d);
+    if (d < p.D) t = *reinterpret_cast<const float4*>(p.part_o + (s * rows + row) * p.D + d);
     sum += f;
     acc.x += f * t.x, acc.y += f * t.y, acc.z += f * t.z, acc.w += f * t.w;
   }
@@ -319,7 +317,7 @@ __global__ void __launch_bounds__(128) ctx_join_kernel(const CtxParams p) {
     acc.x += t.x, acc.y += t.y, acc.z += t.z, acc.w += t.w;
     sum += s_sum[w];
   }
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  const float inv = ctx_inverse(sum);
   if (d < p.D)
     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + row * p.D + d) =
         make_uint2(ctx_pack2<FP16>(acc.x * inv, acc.y * inv), ctx_pack2<FP16>(acc.z * inv, acc.w * inv));
@@ -327,7 +325,7 @@ __global__ void __launch_bounds__(128) ctx_join_kernel(const CtxParams p) {
     const long token = row / p.H;
     const int h = static_cast<int>(row % p.H);
     p.lse[(token / p.Sq * p.H + h) * p.Sq + token % p.Sq] =
-        sum > 0.f ? (mm + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+        ctx_lse2(mm, sum) * 0.6931471805599453f;
   }
 }
 

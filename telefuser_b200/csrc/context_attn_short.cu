@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(CS_WARPS * 32, STEPS == 2 ? 5 : 4) ctx_short_k
         for (int t = 0; t < 2; ++t) mx = fmax3(mx, s[st][t][r * 2], s[st][t][r * 2 + 1]);
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float base = mx == -INFINITY ? 0.f : mx * p.scale_log2;
+      const float top = mx * p.scale_log2, base = ctx_exp_base(top);
       float l = 0.f;
 #pragma unroll
       for (int st = 0; st < STEPS; ++st)
@@ -169,8 +169,8 @@ __global__ void __launch_bounds__(CS_WARPS * 32, STEPS == 2 ? 5 : 4) ctx_short_k
         }
       l += __shfl_xor_sync(0xffffffffu, l, 1);
       l += __shfl_xor_sync(0xffffffffu, l, 2);
-      inv[r] = l > 0.f ? 1.f / l : 0.f;
-      lse2[r] = l > 0.f ? base + log2f(l) : -INFINITY;
+      inv[r] = ctx_inverse(l);
+      lse2[r] = ctx_lse2(top, l);
     }
     long row_at[2];
     bool row_ok[2];

@@ -172,7 +172,7 @@ __device__ __forceinline__ void ctx_new_max(uint32_t tmem_o, float m_new, bool f
   if (first) {
     m_used = m_new;
   } else if (__any_sync(0xffffffffu, (m_new - m_used) > CT_RESCALE_THRESHOLD)) {
-    const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_used - m_new);
+    const float alpha = ctx_rescale(m_used, m_new);
     m_used = m_new;
     l *= alpha;
 #pragma unroll 1
@@ -232,7 +232,7 @@ __device__ __forceinline__ void ctx_softmax_full(uint32_t tmem_s, uint32_t tmem_
     }
   const float mx = fmax3(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]));
   ctx_new_max<DK>(tmem_o, fmaxf(m_used, mx * scale_log2), first, m_used, l);
-  const float neg = m_used == -INFINITY ? 0.f : -m_used;
+  const float neg = -ctx_exp_base(m_used);
   uint64_t ps[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
   for (int c = 0; c < 4; ++c)
@@ -270,7 +270,7 @@ __device__ __forceinline__ void ctx_softmax_part(uint32_t tmem_s, uint32_t tmem_
     }
   }
   ctx_new_max<DK>(tmem_o, fmaxf(m_used, fmaxf(mx0, mx1) * scale_log2), first, m_used, l);
-  const float neg = m_used == -INFINITY ? 0.f : -m_used;
+  const float neg = -ctx_exp_base(m_used);
   uint64_t ps[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll 1
   for (int c = 0; c < chunks; ++c) {
@@ -280,7 +280,7 @@ __device__ __forceinline__ void ctx_softmax_part(uint32_t tmem_s, uint32_t tmem_
   l += ctx_sum(ps);
 }
 
-// An item without keys: zero rows and -inf, or in split form only the mark that its slot saw nothing. Whole warp.
+// An item without keys: zero rows and -inf, in its slot where the key range is split. Whole warp.
 __device__ __noinline__ void ctx_no_keys(const CtxTcParams& p, const CtxItem& t) {
   const int pieces = p.c.D >> 3;  // 16 bytes each
   for (int x = lane_id(); x < 256 * pieces; x += 32) {
@@ -289,7 +289,10 @@ __device__ __noinline__ void ctx_no_keys(const CtxTcParams& p, const CtxItem& t)
     if (tok >= p.c.Sq) break;
     const long token = static_cast<long>(t.b) * p.c.Sq + tok;
     if (p.c.part_o) {
-      if (piece == 0) p.c.part_lse[(static_cast<long>(p.c.slot0 + t.split) * p.c.B * p.c.Sq + token) * p.c.H + head] = -INFINITY;
+      const long at = (static_cast<long>(p.c.slot0 + t.split) * p.c.B * p.c.Sq + token) * p.c.H + head;
+      if (piece == 0) p.c.part_lse[at] = -INFINITY;
+      float4* o = reinterpret_cast<float4*>(p.c.part_o + at * p.c.D) + piece * 2;
+      o[0] = o[1] = make_float4(0.f, 0.f, 0.f, 0.f);
       continue;
     }
     reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.c.out) + (token * p.c.H + head) * p.c.D)[piece] = make_uint4(0, 0, 0, 0);
@@ -384,9 +387,9 @@ __global__ void __launch_bounds__(512, 1)
         const bool row_ok = tok < p.c.Sq;
         if (!(ok = mbar_wait_warp(&l_full[st], (o_phase >> st) & 1, ctx, 56))) break;
         const float2 m_l = ml[st * 128 + row];
-        const float inv = m_l.y > 0.f ? 1.f / m_l.y : 0.f;
+        const float inv = ctx_inverse(m_l.y);
         if (row_ok && (p.c.part_o || p.c.lse)) {
-          const float lse2 = m_l.y > 0.f ? m_l.x + log2f(m_l.y) : -INFINITY;
+          const float lse2 = ctx_lse2(m_l.x, m_l.y);
           if (p.c.part_o)
             p.c.part_lse[((static_cast<long>(p.c.slot0 + t.split) * p.c.B + t.b) * p.c.Sq + tok) * p.c.H + head] = lse2;
           else

@@ -359,3 +359,106 @@ def test_first_block_arrives_last(lib, fp16):
         (k[:, 128:].isnan().sum() + v[:, :128].isnan().sum() + q.isnan().sum())
         o, lse = CA.cross_attention(q, k, v, kv_lens=lens, return_lse=True)
         check(o, lse, want, dtype)
+
+
+# ---- NaN and infinities among the keys that are seen ------------------------------------------------------------------
+SPECIAL = [  # rows kernel without and with a key split, tile kernel without and with one, short kernel
+    (2, 1, 4, 2, 64, 300), (1, 1, 2, 1, 128, 9000), (3, 5, 4, 4, 64, 33), (2, 300, 2, 1, 64, 400), (1, 60, 1, 1, 128, 4000),
+    (1, 200, 2, 2, 128, 2000), (2, 100, 4, 2, 128, 50), (2, 70, 2, 2, 40, 17),
+]
+
+
+def special(t, at, value):
+    t = t.clone()
+    t[at] = value
+    return t
+
+
+def same_kind(got, lse, o64, lse64):
+    """NaN where the definition in 64 bits has NaN, the infinities that it has, and finite values elsewhere."""
+    for a, b in ((got, o64), (lse, lse64)):
+        assert torch.equal(a.isnan(), b.isnan())
+        assert torch.equal(a.double().masked_fill(~a.isinf(), 0), b.masked_fill(~b.isinf(), 0))
+
+
+def special_cases(q, k, v):
+    nan, inf = float("nan"), float("inf")
+    last = k.shape[1] - 1
+    yield "nan in a key", q, special(k, (0, last // 2, 0, 3), nan), v
+    yield "nan in the first key", q, special(k, (0, 0, 0, 3), nan), v
+    yield "inf in a key", q, special(k, (0, last, -1, 0), inf), v
+    yield "-inf in a key", q, special(k, (0, last // 3, 0, 1), -inf), v
+    yield "inf and nan in keys", q, special(special(k, (0, last, 0, 0), inf), (0, 0, 0, 1), nan), v
+    yield "nan in a value", q, k, special(v, (0, last // 2, 0, 3), nan)
+    yield "inf in a value", q, k, special(v, (0, last, 0, 2), inf)
+    yield "nan in a query", special(q, (0, q.shape[1] - 1, 0, 5), nan), k, v
+    yield "inf in a query", special(q, (-1, 0, -1, 5), inf), k, v
+    yield "every key -inf", q.abs(), special(k, (0, slice(None), 0), -inf), v
+    yield "every key -inf, nan in a value", q.abs(), special(k, (0, slice(None), 0), -inf), special(v, (0, last // 2, 0, 3), nan)
+
+
+def definition(q, keys, scale=None):
+    """`exact` with what infinities and NaN do in the sums, as the fp32 evaluation has it: a query whose scores are all -inf
+    has weights of zero."""
+    B, Sq, H, D = q.shape
+    scale = 1.0 / math.sqrt(D) if scale is None else scale
+    out = torch.zeros(B, Sq, H, D, dtype=torch.float64, device=q.device)
+    lse = torch.full((B, H, Sq), float("-inf"), dtype=torch.float64, device=q.device)
+    for b, (k, v) in enumerate(keys):
+        kd, vd = (t.double().repeat_interleave(H // k.shape[1], dim=1).transpose(0, 1) for t in (k, v))
+        s = q[b].double().transpose(0, 1) @ kd.transpose(1, 2) * scale
+        lse[b] = torch.logsumexp(s, dim=-1)
+        p = torch.exp(s - lse[b].masked_fill(lse[b] == float("-inf"), 0.0)[..., None])
+        out[b] = (p @ vd).transpose(0, 1)
+    return out, lse
+
+
+def check_special(q, k, v, dtype):
+    B = q.shape[0]
+    for what, qx, kx, vx in special_cases(q, k, v):
+        want = definition(qx, [(kx[b], vx[b]) for b in range(B)])
+        o, lse = CA.cross_attention(qx, kx, vx, return_lse=True)
+        try:
+            same_kind(o, lse, *want)
+        except AssertionError as e:
+            raise AssertionError(what) from e
+        # rows that come out finite have their values: a key at -inf weighs nothing
+        fine = want[0].isfinite().all(-1)[..., None]
+        _, _, pv, sv, _ = exact(qx, [(kx[b], vx[b]) for b in range(B)])
+        size = exact(q, [(k[b], v[b]) for b in range(B)])[-1]  # finite scores are those of q and k
+        zero = torch.zeros_like(want[0])
+        check(torch.where(fine, o, torch.zeros_like(o)), None, (torch.where(fine, want[0], zero), None,
+              pv.where(fine & pv.isfinite(), zero), sv.where(sv.isfinite(), zero), size), dtype)  # fmt: skip
+
+
+@pytest.mark.parametrize("shape", SPECIAL)
+def test_special_values_on_cpu(shape):
+    q, k, v = make(*shape, torch.float32, "cpu", seed=13)
+    B = q.shape[0]
+    for what, qx, kx, vx in special_cases(q, k, v):
+        o, lse = CA.cross_attention(qx, kx, vx, return_lse=True)
+        same_kind(o, lse, *definition(qx, [(kx[b], vx[b]) for b in range(B)]))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("shape", SPECIAL)
+def test_special_values(lib, shape, dtype):
+    check_special(*make(*shape, dtype, "cuda", seed=13), dtype)
+
+
+@gpu
+@pytest.mark.parametrize("shape,P", [((2, 1, 4, 2, 64, 40), 3000), ((40, 1, 4, 1, 128, 20), 9000), ((2, 130, 2, 2, 64, 90), 140)])
+def test_special_values_in_a_shared_prefix(lib, shape, P):
+    B, Sq, H, Hkv, D, S = shape
+    q, k, v = make(*shape, BF, "cuda", seed=14)
+    _, kp, vp = make(1, 1, 1, Hkv, D, P, BF, "cuda", seed=15)
+    nan, inf = float("nan"), float("inf")
+    for qx, kpx, vpx, kx, vx in [
+        (q, special(kp, (0, P - 1, 0, 2), nan), vp, k, v), (q, kp, vp, special(k, (1, S - 1, 0, 2), nan), v),
+        (special(q, (1, 0, 0, 0), nan), kp, vp, k, v), (q, special(kp, (0, 0, 0, 2), inf), vp, k, v),
+        (q, kp, special(vp, (0, P // 2, 0, 1), nan), k, v), (q, kp, vp, k, special(v, (0, 0, 0, 1), nan)),
+        (q, special(kp, (0, 1, 0, 2), inf), vp, special(k, (0, 0, 0, 1), nan), v),
+    ]:  # fmt: skip
+        o, lse = CA.prefix_attention(qx, kpx, vpx, kx, vx, return_lse=True)
+        same_kind(o, lse, *definition(qx, [(torch.cat([kpx[0], kx[b]]), torch.cat([vpx[0], vx[b]])) for b in range(B)]))
