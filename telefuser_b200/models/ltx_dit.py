@@ -16,6 +16,7 @@ from __future__ import annotations
 import math
 from dataclasses import dataclass, replace
 from enum import Enum
+from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -219,11 +220,26 @@ def _masked_attention(q, k, v, mask):
     return (torch.softmax(s, dim=-1) @ v.float().permute(0, 2, 1, 3)).permute(0, 2, 1, 3).to(q.dtype)
 
 
-def _key_masked_attention(q, k, v, visible):
-    """visible: bool [B, S], True where a context token may be seen. A sample without one attends to all of them evenly, as it
-    does under an additive mask of the lowest finite value."""
+class KeyMask(NamedTuple):
+    """Which context tokens the samples may see, prepared once for all layers (`key_mask`)."""
+
+    seen: torch.Tensor  # bool [B, S]; a sample without a token of its own sees all of them ...
+    some: torch.Tensor  # bool [B, 1, 1, 1]; ... and has False here
+
+
+def key_mask(visible: torch.Tensor, batch: int) -> KeyMask:
+    """visible: bool [B, S], or [1, S] for all samples, True where a context token may be seen."""
     some = visible.any(dim=-1, keepdim=True)
-    return cross_attention(q, torch.where(some[:, :, None, None], k, torch.zeros_like(k)), v, key_mask=visible | ~some)
+    return KeyMask((visible | ~some).expand(batch, -1), some[:, :, None, None])
+
+
+def _key_masked_attention(q, k, v, mask):
+    """mask: a `KeyMask`, or the bool tensor that it is made of. A sample without a visible token attends to all of them evenly,
+    as it does under an additive mask of the lowest finite value. The weights are rounded to the inputs' type for the second
+    product, as in the attention of the same layer without a mask (16-bit inputs; fp32 ones are evaluated in fp32)."""
+    if not isinstance(mask, KeyMask):
+        mask = key_mask(mask, q.shape[0])
+    return cross_attention(q, torch.where(mask.some, k, torch.zeros_like(k)), v, key_mask=mask.seen)
 
 
 class Attention(nn.Module):
@@ -256,7 +272,7 @@ class Attention(nn.Module):
             q4, k4, v4 = q.unflatten(-1, (H, D)), k.unflatten(-1, (H, D)), v.unflatten(-1, (H, D))
             if mask is None:
                 out = TF.attention(q4.contiguous(), k4.contiguous(), v4)
-            elif mask.dtype == torch.bool:
+            elif isinstance(mask, KeyMask) or mask.dtype == torch.bool:
                 out = _key_masked_attention(q4, k4, v4, mask)
             else:
                 out = _masked_attention(q4, k4, v4, mask)
@@ -311,7 +327,7 @@ class Modality:
 class TransformerArgs:
     x: torch.Tensor
     context: torch.Tensor
-    context_mask: torch.Tensor | None
+    context_mask: torch.Tensor | KeyMask | None
     timesteps: torch.Tensor
     embedded_timestep: torch.Tensor
     positional_embeddings: tuple
@@ -514,7 +530,7 @@ class LTXModel(nn.Module):
         cmask = m.context_mask
         if cmask is not None and not torch.is_floating_point(cmask):
             if cmask.numel() == cmask.shape[0] * cmask.shape[-1]:
-                cmask = (cmask > 0).reshape(cmask.shape[0], -1)  # one mark per context token
+                cmask = key_mask((cmask > 0).reshape(cmask.shape[0], -1), B)  # one mark per context token
             else:
                 cmask = (cmask.to(torch.float32) - 1).reshape(cmask.shape[0], 1, -1, cmask.shape[-1]) * torch.finfo(torch.float32).max
         smask = None

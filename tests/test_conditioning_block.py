@@ -97,3 +97,48 @@ def test_ltx_key_masks_equal_the_additive_mask(device):
     # both round the output (2^-8 of it in bf16), and the weights of the kernel's second product 2^-8 of sum p |v| <= max |v|
     tol = 2 * 2.0**-8 * v.float().abs().max().item() if device == "cuda" else 1e-5
     assert ((got.float() - want.float()).abs() <= tol + (2.0**-7 if device == "cuda" else 0) * want.float().abs()).all()
+
+
+# ---- LTX context masks through the model ------------------------------------------------------------------------------
+def ltx_model_and_inputs(B, S, adaln):
+    torch.manual_seed(0)
+    m = LTX.LTXModel(model_type=LTX.LTXModelType.VideoOnly, num_attention_heads=2, attention_head_dim=24, in_channels=8,
+                     out_channels=8, num_layers=2, cross_attention_dim=48, rope_type=LTX.LTXRopeType.SPLIT,
+                     cross_attention_adaln=adaln)  # fmt: skip
+    for p in m.parameters():
+        torch.nn.init.normal_(p, std=0.2)
+    T = 6
+    start = torch.arange(T, dtype=torch.float32)[None, None].expand(B, 3, T)
+    sigma = torch.linspace(0.9, 0.4, B)
+    return m.float().eval(), dict(latent=torch.randn(B, T, 8), sigma=sigma, positions=torch.stack([start, start + 1], dim=-1),
+                                  timesteps=sigma[:, None].expand(B, T), context=torch.randn(B, S, 48))  # fmt: skip
+
+
+@pytest.mark.parametrize("adaln", [False, True])
+@pytest.mark.parametrize("B,mask", [
+    (2, [[0, 0, 1, 1, 1, 0, 1]]),  # one mask for all samples
+    (2, [[0, 0, 1, 1, 1, 0, 1], [1, 1, 1, 1, 0, 0, 0]]),
+    (2, [[0, 0, 0, 0, 0, 0, 0], [1, 0, 0, 0, 0, 0, 0]]),  # a sample without a token
+    (2, [[0, 0, 0, 0, 0, 0, 0]]),
+    (1, [[1, 0, 1, 0, 1, 0, 1]]),
+    (3, [[0, 1, 1, 1, 1, 1, 1]]),
+])  # fmt: skip
+@pytest.mark.parametrize("shape", ["rows", "unit axis", "two unit axes", "bool"])
+def test_ltx_model_context_masks_equal_the_additive_form(B, mask, shape, adaln):
+    m, kw = ltx_model_and_inputs(B, 7, adaln)
+    ones = torch.tensor(mask)
+    additive = (ones.float() - 1)[:, None, None] * torch.finfo(torch.float32).max
+    ones = {"rows": ones, "unit axis": ones[:, None], "two unit axes": ones[:, None, None], "bool": ones.bool()}[shape]
+    want, _ = m(LTX.Modality(context_mask=additive, **kw), None)
+    got, _ = m(LTX.Modality(context_mask=ones, **kw), None)
+    torch.testing.assert_close(got, want, rtol=1e-4, atol=1e-4)
+    if B > 1 and mask != [[0] * 7]:
+        assert not torch.allclose(got, m(LTX.Modality(context_mask=None, **kw), None)[0], atol=1e-3)
+
+
+def test_ltx_model_context_mask_per_query_stays_additive():
+    m, kw = ltx_model_and_inputs(2, 7, False)
+    marks = torch.ones(1, 6, 7, dtype=torch.int64)
+    marks[0, 2:, 3:] = 0
+    want, _ = m(LTX.Modality(context_mask=(marks.float() - 1)[:, None] * torch.finfo(torch.float32).max, **kw), None)
+    torch.testing.assert_close(m(LTX.Modality(context_mask=marks, **kw), None)[0], want)
