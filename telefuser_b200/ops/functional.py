@@ -1148,6 +1148,12 @@ def _row_table(t, shape, rows, C):
     if t is None:
         return None, 0, 0, 1
     n = _table_rows(t, shape, C)
+    if n > 1 and 0 in t.stride():  # expanded views: the rows that repeat are taken once
+        strides = t.stride()
+        if all(m == 1 or st == 0 for m, st in zip(t.shape[:-1], strides[:-1])):
+            t, n = t[(0,) * (t.dim() - 1)], 1
+        elif all(m == 1 or st == 0 for m, st in zip(t.shape[1:-1], strides[1:-1])):
+            t, n = t[(slice(None),) + (0,) * (t.dim() - 2)], t.shape[0]
     if t.dtype != torch.float32:
         t = t.float()
     at = t.data_ptr()

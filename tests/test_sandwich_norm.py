@@ -156,3 +156,34 @@ def test_same_bits_again_and_replayed():
     torch.cuda.synchronize()
     assert torch.equal(x, xg) and torch.equal(h, hg)
     assert native.last_status() == 0
+
+
+# ---- expanded tables --------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("base,shape,rows_per", [
+    ((1, 1, 32), (1, 37, 32), 37), ((1, 1, 32), (3, 37, 32), 111), ((3, 1, 32), (3, 37, 32), 37), ((32,), (3, 37, 32), 111),
+    ((1, 1, 32), (3, 1, 32), 111), ((3, 37, 32), (3, 37, 32), 1), ((1, 37, 32), (3, 37, 32), 1), ((1, 37, 32), (1, 37, 32), 1),
+    ((1, 1, 1), (3, 37, 32), 111), ((3, 37, 1), (3, 37, 32), 1),
+])  # fmt: skip
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_that_an_expanded_table_repeats_are_taken_once(base, shape, rows_per, dtype):
+    acts = torch.empty(3, 37, 32) if shape[0] == 3 else torch.empty(1, 37, 32)
+    rows = acts.numel() // 32
+    wide = torch.randn(*base[:-1], 2 * base[-1] if base[-1] > 1 else 1).to(dtype)
+    view = wide[..., : base[-1]].expand(shape)  # a slice of a wider table, expanded
+    t, at, ld, per = TF._row_table(view, acts.shape, rows, 32)
+    assert per == rows_per and ld % 4 == 0 and at % 16 == 0 and at == t.data_ptr()
+    flat = torch.as_strided(t, (rows // per, 32), (ld, 1))
+    assert torch.equal(flat.repeat_interleave(per, dim=0), view.float().expand(acts.shape).reshape(rows, 32))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_expanded_tables(dtype):
+    a = inputs(3, 500, 264, dtype, "cuda")
+    small = {k: a[k].clone() for k in ("gate", "shift", "scale")}
+    a["gate"], a["shift"] = small["gate"].expand(3, 500, 264), small["shift"][:1].expand(3, 500, 264)
+    a["scale"] = small["scale"][:1].expand(3, 1, 264)
+    x, h = TF.rmsnorm_gate_residual_modulate(**a)
+    check(x, h, a)
+    b = a | dict(gate=small["gate"], shift=small["shift"][:1], scale=small["scale"][:1])
+    assert all(torch.equal(s, t) for s, t in zip((x, h), TF.rmsnorm_gate_residual_modulate(**b)))
