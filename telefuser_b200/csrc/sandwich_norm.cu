@@ -514,11 +514,17 @@ static int launch_snorm_warp(const SnormParams& p, long per_sample, cudaStream_t
   return cudaGetLastError() == cudaSuccess ? TFB_OK : TFB_ERR_LAUNCH;
 }
 
-// Warp per row: per-sample tables, 16-bit rows of up to 5120 columns (so that six rows and the tables fit), and rows enough
-// for eight warps on every SM.
+// Warp per row: per-sample tables, 16-bit rows of up to 5120 columns (so that six rows and the tables fit), rows enough for
+// eight warps on every SM, and eight rows or more under one table row: a CTA there folds the tables of one sample only. bf16, CTA
+// per row against warp per row: 1000 x 2 rows of 2048 14.0 and 31.0 us, 4000 x 7 114 and 144, 1000 x 8 39 and 41, 148 x 8 8.1 and
+// 6.2, 500 x 16 35.8 and 35.4, 500 x 60 98 and 87. Above 4096 columns, where a CTA per row needs two column groups per thread, warps
+// are no slower with any number: 1000 x 2 rows of 5120 66 and 66, 500 x 4 47 and 39, 4000 x 7 446 and 286. 75 .. 147 samples get a
+// CTA each and leave the other SMs idle, which is still as fast as a CTA per row (75 x 400 rows: 1024 columns 54.4 and 53.9,
+// 2048 96 and 101, 3840 172 and 187, 5120 300 and 303; 75 x 32 of 2048 15.2 and 12.0).
 template <typename T>
 static bool snorm_by_warps(const SnormParams& p) {
-  return sizeof(T) == 2 && !p.token && p.C <= 5120 && p.rows >= 8L * sm_count() && p.rows <= 0x7fffffffL;
+  return sizeof(T) == 2 && !p.token && p.C <= 5120 && p.rows >= 8L * sm_count() && p.rows <= 0x7fffffffL &&
+         (p.rp >= 8 || p.C > 4096);
 }
 
 template <typename T>

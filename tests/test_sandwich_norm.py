@@ -187,3 +187,13 @@ def test_expanded_tables(dtype):
     check(x, h, a)
     b = a | dict(gate=small["gate"], shift=small["shift"][:1], scale=small["scale"][:1])
     assert all(torch.equal(s, t) for s, t in zip((x, h), TF.rmsnorm_gate_residual_modulate(**b)))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,S,C", [(1200, 1, 264), (600, 2, 2048), (700, 3, 1024), (301, 4, 3840), (211, 7, 520), (211, 8, 520), (300, 4, 5120), (600, 2, 4104), (75, 17, 1024)])
+def test_many_samples_of_few_rows(B, S, C, dtype):
+    a = inputs(B, S, C, dtype, "cuda")
+    check(*TF.rmsnorm_gate_residual_modulate(**a), a)
+    one = a | dict(gate=a["gate"][:1].expand(B, S, C), shift=a["shift"][:1], scale=a["scale"].expand(B, S, C))
+    check(*TF.rmsnorm_gate_residual_modulate(**one), one)
