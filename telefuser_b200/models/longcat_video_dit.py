@@ -74,10 +74,13 @@ class Attention(nn.Module):
             q, k, v = (ulysses.scatter_heads(t.contiguous(), group) for t in (q, k, v))
         new_cache = (k.clone(), v.clone()) if return_kv else None
         if kv_cache is not None:
-            ck, cv = (c.to(k.device) for c in kv_cache)
-            if ck.shape[0] == 1:  # one clean clip for all samples (guidance branches): read in place
+            # the kernels read one type; the fp32 evaluation on the CPU takes kept keys as they are
+            ck, cv = (c.to(k) if k.is_cuda else c.to(k.device) for c in kv_cache)
+            if ck.shape[0] == 1 and ck.dtype == k.dtype:  # one clean clip for all samples (guidance branches): read in place
                 o = prefix_attention(q, ck, cv, k, v)
-            else:
+            else:  # a clip per sample, or keys kept in another type
+                if ck.shape[0] == 1:
+                    ck, cv = ck.expand(B, -1, -1, -1), cv.expand(B, -1, -1, -1)
                 o = TF.attention(q, torch.cat([ck, k], dim=1), torch.cat([cv, v], dim=1))
         elif num_cond_latents and num_cond_latents > 0:
             n_cond = num_cond_latents * (q.shape[1] // shape[0])

@@ -142,3 +142,31 @@ def test_ltx_model_context_mask_per_query_stays_additive():
     marks[0, 2:, 3:] = 0
     want, _ = m(LTX.Modality(context_mask=(marks.float() - 1)[:, None] * torch.finfo(torch.float32).max, **kw), None)
     torch.testing.assert_close(m(LTX.Modality(context_mask=marks, **kw), None)[0], want)
+
+
+@pytest.mark.parametrize("B", [1, 2])
+@pytest.mark.parametrize("kept,running", [(torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16), (torch.float64, torch.float32)])
+def test_longcat_cached_clip_of_another_type(B, kept, running):
+    """Keys that were kept in one type under a model that runs in another join in the wider of the two."""
+    torch.manual_seed(0)
+    m = LC.Attention(32, 4).to(running)
+    x = torch.randn(B, 6, 32).to(running)
+    rope = (torch.ones(6, 4), torch.zeros(6, 4))
+    cache = tuple(torch.randn(1, 7, 4, 8).to(kept) for _ in range(2))
+    got, _ = m(x, rope, kv_cache=cache)
+    want, _ = m(x, rope, kv_cache=tuple(c.to(torch.promote_types(kept, running)).expand(B, -1, -1, -1).clone() for c in cache))
+    assert got.dtype == running
+    u = torch.finfo(running).eps  # both round their output once, from evaluations in fp32 of the same values
+    torch.testing.assert_close(got, want, rtol=u, atol=1e-5 if running == torch.float32 else u)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [1, 2])
+def test_longcat_cached_clip_of_another_type_on_gpu(B):
+    torch.manual_seed(0)
+    m = LC.Attention(256, 2).to("cuda", torch.bfloat16)
+    x = torch.randn(B, 70, 256, device="cuda", dtype=torch.bfloat16)
+    rope = (torch.ones(70, 64, device="cuda"), torch.zeros(70, 64, device="cuda"))
+    cache = tuple(torch.randn(1, 90, 2, 128, device="cuda") for _ in range(2))
+    got, _ = m(x, rope, kv_cache=cache)
+    assert torch.equal(got, m(x, rope, kv_cache=tuple(c.bfloat16() for c in cache))[0])
