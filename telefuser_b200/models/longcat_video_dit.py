@@ -106,8 +106,8 @@ class MultiHeadCrossAttention(nn.Module):
         self.q_norm, self.k_norm = _WeightOnly(self.head_dim), _WeightOnly(self.head_dim)
 
     def forward(self, x, cond, kv_seqlen):
-        """x [B, N, C]; cond [1, sum of lengths, C], the valid text tokens of all samples in a row; kv_seqlen: the lengths, or
-        their running sum from 0 as an int32 tensor [B + 1] on x's device (see `text_offsets`)."""
+        """x [B, N, C]; cond [1, sum of lengths, C], the valid text tokens of all samples in a row; kv_seqlen: the B lengths (numbers
+        or a tensor), or their running sum from 0 as an int32 tensor [B + 1] on x's device (see `text_offsets`)."""
         B, N, C = x.shape
         H, D = self.num_heads, self.head_dim
         q = TF.linear(x, self.q_linear.weight, self.q_linear.bias).unflatten(-1, (H, D))
@@ -115,13 +115,20 @@ class MultiHeadCrossAttention(nn.Module):
         k, v = kv[..., :C].unflatten(-1, (H, D)), kv[..., C:].unflatten(-1, (H, D))
         TF.headnorm_rope_(q, self.q_norm.weight, None, None, 1e-6)
         TF.headnorm_rope_(k, self.k_norm.weight, None, None, 1e-6)
-        cu = kv_seqlen if torch.is_tensor(kv_seqlen) else text_offsets(kv_seqlen, x.device)
+        cu = kv_seqlen if torch.is_tensor(kv_seqlen) and kv_seqlen.shape == (B + 1,) else text_offsets(kv_seqlen[:B], x.device)
         return cross_attention(q, k, v, cu_kv=cu).reshape(B, N, C)  # every sample sees only its own text tokens
 
 
 def text_offsets(lengths, device) -> torch.Tensor:
-    """int32 [B + 1]: where each sample's text tokens begin in the packed row, and the end of the last."""
-    return torch.tensor([0, *itertools.accumulate(int(n) for n in lengths)], dtype=torch.int32, device=device)
+    """int32 [B + 1]: where each sample's text tokens begin in the packed row, and the end of the last. Numbers reach a GPU as the
+    arguments of fills: copying them from the host would wait for the stream and could not be captured in a graph."""
+    if torch.is_tensor(lengths):
+        return F.pad(lengths.to(device).cumsum(0), (1, 0)).to(torch.int32)
+    ends = list(itertools.accumulate(int(n) for n in lengths))
+    offsets = torch.zeros(len(ends) + 1, dtype=torch.int32, device=device)
+    for i, end in enumerate(ends):
+        offsets[i + 1].fill_(end)
+    return offsets
 
 
 class FeedForwardSwiGLU(nn.Module):

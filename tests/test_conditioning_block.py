@@ -170,3 +170,29 @@ def test_longcat_cached_clip_of_another_type_on_gpu(B):
     cache = tuple(torch.randn(1, 90, 2, 128, device="cuda") for _ in range(2))
     got, _ = m(x, rope, kv_cache=cache)
     assert torch.equal(got, m(x, rope, kv_cache=tuple(c.bfloat16() for c in cache))[0])
+
+
+def test_longcat_text_lengths_as_a_tensor():
+    torch.manual_seed(0)
+    m = LC.MultiHeadCrossAttention(32, 4)
+    x, cond = torch.randn(3, 5, 32), torch.randn(1, 9, 32)
+    want = m(x, cond, [4, 0, 5])
+    assert torch.equal(m(x, cond, torch.tensor([4, 0, 5])), want)
+    assert torch.equal(m(x, cond, (4, 0, 5, 7)), want)  # one length per sample is looked at
+    assert LC.text_offsets([4, 0, 5], "cpu").tolist() == LC.text_offsets(torch.tensor([4, 0, 5]), "cpu").tolist() == [0, 4, 4, 9]
+
+
+@pytest.mark.gpu
+def test_longcat_text_attention_in_a_captured_graph():
+    """Lengths given as numbers need no copy from the host, so the call can be captured."""
+    torch.manual_seed(0)
+    m = LC.MultiHeadCrossAttention(256, 2).to("cuda", torch.bfloat16)
+    x, cond = torch.randn(2, 70, 256, device="cuda").bfloat16(), torch.randn(1, 30, 256, device="cuda").bfloat16()
+    with torch.no_grad():
+        want = m(x, cond, [19, 11])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = m(x, cond, [19, 11])
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
