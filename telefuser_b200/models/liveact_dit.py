@@ -59,6 +59,8 @@ class SingleStreamAttention(nn.Module):
         first = start_f + (self.sp_rank * n_t if self.sp_flag else 0)
         kv = TF.linear(enc[first : first + n_t].to(xf.dtype), self.kv_linear.weight, self.kv_linear.bias)
         k, v = kv[..., :C].unflatten(-1, (H, D)), kv[..., C:].unflatten(-1, (H, D))
+        if k.shape[0] == 1 < B0 * n_t:  # one audio window for all frames
+            k, v = k.expand(B0 * n_t, -1, -1, -1), v.expand(B0 * n_t, -1, -1, -1)
         o = cross_attention(q, k, v).reshape(B0 * n_t, S, C)
         return TF.linear(o, self.proj.weight, self.proj.bias).reshape(B0, N, C)
 

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from telefuser_b200.models import liveact_dit as LA
 from telefuser_b200.models import longcat_video_dit as LC
 from telefuser_b200.models import ltx_dit as LTX
 from telefuser_b200.ops import context_attention as CA
@@ -196,3 +197,16 @@ def test_longcat_text_attention_in_a_captured_graph():
         graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("B,n_t", [(1, 3), (2, 1), (2, 3)])
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_liveact_one_audio_window_serves_every_frame(B, n_t, device):
+    torch.manual_seed(0)
+    dt = torch.bfloat16 if device == "cuda" else torch.float32
+    m = LA.SingleStreamAttention(64, 48, 4).to(device, dt)
+    x, enc = torch.randn(B, n_t * 6, 64).to(device, dt), torch.randn(1, 4, 5, 48).to(device, dt)
+    got = m(x, enc, (n_t, 2, 3), start_f=3)  # only the last window is left
+    frames = x.reshape(B * n_t, 6, 64)
+    want = torch.cat([m(f[None], enc[:, 3:], (1, 2, 3)) for f in frames]).reshape(B, n_t * 6, 64)
+    torch.testing.assert_close(got, want, rtol=torch.finfo(dt).eps, atol=torch.finfo(dt).eps)
