@@ -33,6 +33,9 @@ def context_attention_reference(q, k, v, visible=None, scale=None, return_lse=Fa
     """fp32 evaluation: q [B, Sq, H, D], k / v [B, Skv, Hkv, D] (H a multiple of Hkv), visible bool [B, Skv] or None."""
     B, Sq, H, D = q.shape
     Skv, Hkv = k.shape[1], k.shape[2]
+    if 0 in (B, Sq, H):
+        out, lse = torch.empty_like(q), q.new_empty(B, H, Sq, dtype=torch.float32)
+        return (out, lse) if return_lse else out
     scale = 1.0 / math.sqrt(D) if scale is None else scale
     kf, vf = k.float().permute(0, 2, 3, 1), v.float().transpose(1, 2)  # [B, Hkv, D, Skv], [B, Hkv, Skv, D]
     if visible is not None:  # hidden rows may hold anything
@@ -193,8 +196,8 @@ def cross_attention(q, k, v, kv_lens=None, cu_kv=None, key_mask=None, scale=None
     if cu_kv is not None:
         cu = [min(max(x, 0), Skv) for x in cu_kv.tolist()]
         lens = [max(b - a, 0) for a, b in zip(cu, cu[1:])]
-        at = torch.tensor(cu[:-1], device=q.device)[:, None] + torch.arange(max(lens, default=0), device=q.device)
-        visible = torch.arange(at.shape[1], device=q.device) < torch.tensor(lens, device=q.device)[:, None]
+        at = torch.tensor(cu[:-1], dtype=torch.long, device=q.device)[:, None] + torch.arange(max(lens, default=0), device=q.device)
+        visible = torch.arange(at.shape[1], device=q.device) < torch.tensor(lens, dtype=torch.long, device=q.device)[:, None]
         k, v = (t[0][at.clamp(max=max(Skv - 1, 0))] if Skv else t.new_zeros(B, 0, *t.shape[2:]) for t in (k, v))
     elif kv_lens is not None:
         seen = torch.arange(Skv, device=q.device) < kv_lens[:, None]

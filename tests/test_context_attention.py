@@ -462,3 +462,19 @@ def test_special_values_in_a_shared_prefix(lib, shape, P):
     ]:  # fmt: skip
         o, lse = CA.prefix_attention(qx, kpx, vpx, kx, vx, return_lse=True)
         same_kind(o, lse, *definition(qx, [(torch.cat([kpx[0], kx[b]]), torch.cat([vpx[0], vx[b]])) for b in range(B)]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF])
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("B,Sq,H", [(0, 3, 4), (2, 0, 4), (2, 3, 0), (0, 0, 0)])
+def test_empty_queries_give_empty_results(B, Sq, H, device, dtype):
+    q, k, v = make(B, Sq, H, 2, 8, 5, dtype, device)
+    _, kp, vp = make(1, 1, 1, 2, 8, 7, dtype, device)
+    packed = [t.reshape(-1, 2, 8) for t in (k, v)]
+    cu = torch.arange(B + 1, device=device) * 5
+    for o, lse in [
+        CA.cross_attention(q, k, v, return_lse=True), CA.cross_attention(q, k, v, kv_lens=[3] * B, return_lse=True),
+        CA.cross_attention(q, k, v, key_mask=torch.ones(B, 5, dtype=torch.bool, device=device), return_lse=True),
+        CA.cross_attention(q, *packed, cu_kv=cu, return_lse=True), CA.prefix_attention(q, kp, vp, k, v, return_lse=True),
+    ]:  # fmt: skip
+        assert o.shape == (B, Sq, H, 8) and o.dtype == dtype and lse.shape == (B, H, Sq) and lse.dtype == torch.float32
