@@ -78,8 +78,8 @@ def _check(q, k, v, what: str) -> None:
 
 def _scale(scale, D: int) -> float:
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
-        raise ValueError("the score scale must be positive and finite")
+    if not 2.0**-126 <= scale <= 2.0**127:  # the kernels hold it, times log2(e), in fp32
+        raise ValueError(f"the score scale must be positive, finite and a normal number in fp32, got {scale}")
     return scale
 
 

@@ -478,3 +478,13 @@ def test_empty_queries_give_empty_results(B, Sq, H, device, dtype):
         CA.cross_attention(q, *packed, cu_kv=cu, return_lse=True), CA.prefix_attention(q, kp, vp, k, v, return_lse=True),
     ]:  # fmt: skip
         assert o.shape == (B, Sq, H, 8) and o.dtype == dtype and lse.shape == (B, H, Sq) and lse.dtype == torch.float32
+
+
+@pytest.mark.parametrize("scale", [1e39, 1e-39, 1e-60, float("inf"), 2.0**127.5])
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_scales_beyond_fp32_are_refused(scale, device):
+    q, k, v = make(2, 3, 4, 2, 8, 7, BF, device)
+    with pytest.raises(ValueError, match="scale"):
+        CA.cross_attention(q, k, v, scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        CA.prefix_attention(q, k[:1], v[:1], k, v, scale=scale)
