@@ -86,10 +86,10 @@ def _scale(scale, D: int) -> float:
 def _lengths(lens, n: int, most: int, device, what: str):
     """-> int32 [n] on `device`. Values that the host holds are checked; values on the device are clamped by the kernels."""
     if not torch.is_tensor(lens) or lens.device.type == "cpu":
-        values = [int(x) for x in lens]
-        if len(values) != n or any(not 0 <= x <= most for x in values):
-            raise ValueError(f"{what}: {n} values in [0, {most}] expected, got {values}")
-        return torch.tensor(values, dtype=torch.int32, device=device)
+        values = lens.tolist() if torch.is_tensor(lens) else list(lens)
+        if len(values) != n or any(isinstance(x, list) or x != int(x) or not 0 <= x <= most for x in values):
+            raise ValueError(f"{what}: {n} whole numbers in [0, {most}] expected, got {values}")
+        return torch.tensor([int(x) for x in values], dtype=torch.int32, device=device)
     if lens.shape != (n,) or lens.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{what}: an integer tensor of shape ({n},) expected, got {lens.dtype} {tuple(lens.shape)}")
     if lens.device != device:

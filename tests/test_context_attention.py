@@ -488,3 +488,18 @@ def test_scales_beyond_fp32_are_refused(scale, device):
         CA.cross_attention(q, k, v, scale=scale)
     with pytest.raises(ValueError, match="scale"):
         CA.prefix_attention(q, k[:1], v[:1], k, v, scale=scale)
+
+
+@pytest.mark.parametrize("lens", [[2.5, 3], torch.tensor([2.0, 3.25]), torch.tensor([[2], [3]]), torch.tensor([[2, 3]])])
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_lengths_that_are_no_whole_numbers_are_refused(lens, device):
+    q, k, v = make(2, 3, 4, 2, 8, 7, BF, device)
+    with pytest.raises(ValueError):
+        CA.cross_attention(q, k, v, kv_lens=lens)
+    with pytest.raises(ValueError):
+        CA.prefix_attention(q, k[:1], v[:1], k, v, kv_lens=lens)
+    with pytest.raises(ValueError):
+        CA.cross_attention(q, k[0], v[0], cu_kv=torch.tensor([0.0, 2.5, 7.0]))
+    kept = CA.cross_attention(q, k, v, kv_lens=[2, 3])
+    for same in ((2, 3), torch.tensor([2, 3]), [torch.tensor(2), torch.tensor(3)], torch.tensor([2.0, 3.0]), range(2, 4)):
+        assert torch.equal(CA.cross_attention(q, k, v, kv_lens=same), kept)
