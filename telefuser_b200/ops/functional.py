@@ -1220,9 +1220,8 @@ def rmsnorm_gate_residual_modulate(res, y, weight=None, gate=None, next_weight=N
     native.same_device(res, y, weight, gate, next_weight, shift, scale)
     kind = _SNORM_TYPES.get(dtype)
     if kind is None or not _native(res) or C % 8 or C > 8192:
-        for t in (gate, shift, scale):
-            if t is not None:
-                _table_rows(t, shape, C)
+        # one row for all keeps the activations' shape whatever its own
+        gate, shift, scale = (t if t is None or _table_rows(t, shape, C) != 1 else t.reshape(C) for t in (gate, shift, scale))
         n = _rms(y, weight, eps) if post_norm else y.float()
         if gate is not None:
             n = (gate.float().tanh() if tanh_gate else gate.float()) * n

@@ -197,3 +197,23 @@ def test_many_samples_of_few_rows(B, S, C, dtype):
     check(*TF.rmsnorm_gate_residual_modulate(**a), a)
     one = a | dict(gate=a["gate"][:1].expand(B, S, C), shift=a["shift"][:1], scale=a["scale"].expand(B, S, C))
     check(*TF.rmsnorm_gate_residual_modulate(**one), one)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("shape", [(24,), (5, 24), (2, 5, 24)])
+@pytest.mark.parametrize("extra", [0, 1, 3])
+def test_one_row_for_all_keeps_the_shape_of_the_activations(shape, extra, device):
+    g = torch.Generator().manual_seed(0)
+    a = {n: torch.randn(*shape, generator=g).to(device) for n in ("res", "y")}
+    a |= {n: torch.randn(*(1,) * extra, 24, generator=g).to(device) for n in ("gate", "shift", "scale")} | dict(weight=None, next_weight=None)
+    x, h = TF.rmsnorm_gate_residual_modulate(**a)
+    assert x.shape == h.shape == shape
+    check(x, h, {k: v.reshape(24) if k in ("gate", "shift", "scale") else v for k, v in a.items()})
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("shape,table", [((0, 5, 24), (0, 1, 24)), ((0, 5, 24), (1, 1, 24)), ((2, 0, 24), (2, 1, 24)), ((2, 0, 24), (2, 0, 24))])
+def test_empty_activations_with_tables(shape, table, device):
+    z = torch.zeros(shape, device=device)
+    x, h = TF.rmsnorm_gate_residual_modulate(z, z, gate=torch.zeros(table, device=device), scale=torch.zeros(24, device=device))
+    assert x.shape == h.shape == shape
