@@ -503,3 +503,44 @@ def test_lengths_that_are_no_whole_numbers_are_refused(lens, device):
     kept = CA.cross_attention(q, k, v, kv_lens=[2, 3])
     for same in ((2, 3), torch.tensor([2, 3]), [torch.tensor(2), torch.tensor(3)], torch.tensor([2.0, 3.0]), range(2, 4)):
         assert torch.equal(CA.cross_attention(q, k, v, kv_lens=same), kept)
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(2, 1, 8, 2, 128, 5000), (1, 300, 2, 2, 128, 3000), (30, 1, 8, 2, 64, 900)])
+def test_split_calls_that_overlap_do_not_share_scratch(lib, shape):
+    """Calls with a split key range and inputs of their own on two streams without an order between them, then two captured
+    graphs replayed on the two: every result is that of the call alone."""
+    B, Sq, H, Hkv, D, Skv = shape
+    sides = []
+    for seed in (21, 22):
+        q, k, v = make(*shape, BF, "cuda", seed=seed)
+        _, kp, vp = make(1, 1, 1, Hkv, D, 4000, BF, "cuda", seed=seed + 10)
+        sides.append((q, k, v, kp, vp))
+
+    def calls(q, k, v, kp, vp):
+        return *CA.cross_attention(q, k, v, return_lse=True), *CA.prefix_attention(q, kp, vp, k, v, return_lse=True)
+
+    alone = [calls(*s) for s in sides]
+    assert not torch.equal(alone[0][0], alone[1][0])
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(30):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(calls(*sides[i]))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        assert all(torch.equal(a, b) for r in got[i] for a, b in zip(r, alone[i]))
+    graphs, outs = [], []
+    for s in sides:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(calls(*s))
+    for _ in range(30):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        assert all(torch.equal(a, b) for a, b in zip(outs[i], alone[i]))
