@@ -1,8 +1,20 @@
 // C entry points of context attention: argument checks, the choice of kernels and key splits.
 //
-// Rows kernel (context_attn_rows.cu) when a sample has at most 32 query rows per key head (20 rows x 8 key heads against 131072
-// keys: 97 us there, 119 in a query tile of the tensor-memory kernel); otherwise the short-state kernel
-// (context_attn_short.cu) up to 64 key rows in all and the tensor-memory kernel (context_attn_tc.cu) beyond.
+// Rows kernel (context_attn_rows.cu) when a sample has at most 32 query rows per key head; otherwise the short-state kernel
+// (context_attn_short.cu) up to 64 key rows in all and the tensor-memory kernel (context_attn_tc.cu) beyond. Both sides of the
+// limit, 8 key heads, bf16, us in the rows kernel and in the one that would run without it:
+//            head dim 64                                          head dim 128
+//   keys     B  1: 1 row     17 rows    32 rows                   1 row       17 rows    32 rows
+//   128      4.2 / 7.6       6.0 / 7.6    6.6 / 7.4                4.8 / 8.3     7.9 / 8.3    9.3 / 8.4
+//   2048     9.8 / 12.1     13.4 / 12.5  14.0 / 12.4              11.5 / 13.0   16.9 / 13.2  18.7 / 13.1
+//   32768   16.9 / 31.9     24.4 / 32.5  25.5 / 32.6              29.8 / 45.3   37.1 / 45.5  38.3 / 44.1
+//            B 64
+//   128      8.3 / 16.9     13.0 / 16.9  14.6 / 16.8              10.2 / 19.8   18.6 / 19.8  22.8 / 19.9
+//   2048    52.2 / 103      77.1 / 104   79.9 / 104               80.9 / 126     101 / 126    107 / 126
+//   8192     177 / 378       258 / 378    262 / 378                301 / 463     348 / 474    368 / 504
+// The limit is right where the call takes long; below 15 us it costs up to 30 % with more than 16 rows, and up to 64 keys the
+// short-state kernel would be faster for 16 rows and more (32 keys, 16 and 32 rows of B 64 at head dim 64: 8.1 / 4.5 and
+// 12.1 / 4.7; 1 row of B 1 at head dim 128: 3.9 / 4.6).
 // A shared prefix is visited as the first keys of every sample while re-reading it costs little: always when a sample fills a
 // query tile, and below that while the batch's re-reads stay small enough for L2. Otherwise it is computed once for all
 // samples - their tokens form one batch entry - as slots of its own, the samples' own keys as further slots, and the join

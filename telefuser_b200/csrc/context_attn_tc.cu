@@ -22,10 +22,13 @@
 // its view of an item is four integers. (An issuer per tile was slower, 594 for 558 us on two prompts of 512 and 183 tokens:
 // the tensor core takes turns between two warps, and both tiles' chains get longer.)
 //
-// Measured: 2 x 3120 tokens x 32 heads of 128 against a prefix of 9360 and 3120 own keys 1130 us, 1130 TFLOP/s, where the MMAs
-// and their hand-overs alone take about 1000; two prompts of 512 and 183 keys under 37440 tokens x 32 heads 525 us, 810 TFLOP/s, where
-// the ends of the short items (first Q.K^T, last P.V, hand-over to the output warps) leave tensor pipe and exponentials at 40 %
-// each.
+// Measured, replayed from a graph: 2 x 3120 tokens x 32 heads of 128 against a prefix of 9360 and 3120 own keys 1130 us, 1130
+// TFLOP/s, where the MMAs and their hand-overs alone take about 1000; two prompts of 512 and 183 keys under 37440 tokens x 32 heads
+// 525 us, 810 TFLOP/s, where the ends of the short items (first Q.K^T, last P.V, hand-over to the output warps) leave tensor pipe and
+// exponentials at 40 % each. (On a board that reached its power cap sooner 1313 and 606 us.)
+// Head groups that are no power of two, or larger than 32, fill a tile with one head's tokens and read K and V once per head: 8 samples
+// x 12 tokens x 3 heads per key head against 4096 keys take 121 us, with 4 heads per key head 46; 100 tokens 122 and 72. From a
+// few hundred tokens on it makes no difference (1000 tokens, 3 and 4 heads: 385 and 482).
 //
 // The row maximum that exp2 uses is only raised when it grew by more than 2^8. P is rounded to the inputs' type for the
 // product (at most 2^8, sum in fp32).

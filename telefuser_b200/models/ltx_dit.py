@@ -7,7 +7,7 @@ on queries and on the prompt), bidirectional audio<->video cross-attention with 
 time axis and timestep-driven scale / shift / gate tables, and a GELU-tanh MLP. Guidance perturbations can skip
 a block's self- or cross-modal attention per sample (a skipped self-attention passes the value projection).
 The modulated norms, the MLP (activation and gate * y + residual in the GEMM epilogues) and attention run on the
-native kernels; the full-width rotary embedding and the masked forms use PyTorch.
+native kernels, masks with one mark per context token included; the full-width rotary embedding and additive masks use PyTorch.
 Role parity: telefuser/models/ltx_dit.py:84-2227.
 """
 

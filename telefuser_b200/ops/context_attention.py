@@ -7,8 +7,9 @@ CUDA bf16 / fp16 tensors with a head dim that is a multiple of 8 up to 128 run o
 everything else (CPU, fp32, other head dims) takes the fp32 evaluation of `context_attention_reference`, in query blocks.
 
 A query that sees no key gives a zero row, and -inf as its log-sum-exp. What lies in padded or masked places does not
-matter, infinities and NaN included. Inference only: no gradient is recorded. Neither call synchronises with the host when
-lengths are given as device tensors, so both can be captured in a CUDA graph.
+matter, infinities and NaN included; what lies in visible ones reaches the results as in a plain evaluation. Inference only: the kernels
+record no gradient. On the kernels neither call synchronises with the host when lengths are given as device tensors, so both
+can be captured in a CUDA graph (the fp32 evaluation reads `cu_kv` on the host).
 
 Role parity: telefuser/ops/attention/attention_impl.py:112-315 (variable-length forms of the attention back ends).
 """
