@@ -776,6 +776,9 @@ int launch_ctx_tc(const CtxParams& c, int fp16, cudaStream_t st) {
   if (items > 0x3fffffffL) return TFB_ERR_TOO_LARGE;
   // An item takes about 2 us per 128 keys, and the output warps wait for all of it: well inside their bounded wait (0.8 s).
   if ((static_cast<long>(c.Skv) + c.P) / c.ns > (1L << 24)) return TFB_ERR_TOO_LARGE;
+  // Nor may the decoder keep the other warps waiting: it passes over the masks of samples that see nothing at about 512 bytes a
+  // microsecond, and one CTA may meet those of all samples in a row.
+  if (c.key_mask && static_cast<long>(c.B) * c.Skv > (1L << 27)) return TFB_ERR_TOO_LARGE;
   p.n_items = static_cast<int>(items);
   CUtensorMap tm[6];
   const int kb = packed ? 1 : c.B;

@@ -544,3 +544,17 @@ def test_split_calls_that_overlap_do_not_share_scratch(lib, shape):
     torch.cuda.synchronize()
     for i in (0, 1):
         assert all(torch.equal(a, b) for a, b in zip(outs[i], alone[i]))
+
+
+@gpu
+def test_masks_too_long_for_the_bounded_waits_are_refused(lib):
+    """One sample more than the limit; the largest masks below it are accepted, all hidden and all visible."""
+    Skv, D = 1 << 23, 8
+    kv = torch.zeros(17, Skv, 1, D, device="cuda", dtype=BF)
+    q = torch.zeros(17, 40, 1, D, device="cuda", dtype=BF)
+    for shown in (False, True):
+        mask = torch.full((1, Skv), shown, device="cuda").expand(17, -1)
+        with pytest.raises(native.NativeLibraryError):
+            CA.cross_attention(q, kv, kv, key_mask=mask)
+        o, lse = CA.cross_attention(q[:16], kv[:16], kv[:16], key_mask=mask[:16], return_lse=True)
+        assert (o == 0).all() and ((lse - math.log(Skv)).abs() < 1e-4 if shown else lse == float("-inf")).all()
